@@ -388,6 +388,137 @@ int tcrv_cuda_gemm_q4_0_q8_0_static_scratch(size_t n, float *s, const uint8_t *v
                                             size_t nr, size_t nc, size_t bx, size_t bs, unsigned flags,
                                             tcrv_cuda_stream stream);
 
+/* ---- attention over a paged Q4_0 key/value cache -------------------------------------------
+ * What lies between a decoder layer's projections in a serving step: which slots the step's new
+ * tokens get, rotary positions, the cache's writer, and attention over it.  The reference has none
+ * of these operations.  Activations are f32, fp16 or bf16; every sum, soft-max statistic and
+ * rotation is f32 or wider.  No entry allocates; all may be captured into a graph. */
+#define TCRV_CUDA_TYPE_F32 0
+#define TCRV_CUDA_TYPE_F16 1
+#define TCRV_CUDA_TYPE_BF16 2
+
+/* Rotary positions of any number of tokens.  Pair p < n_rot / 2 of every head of token i turns by
+ * the angle positions[i] * freqs[p], computed in 64 bits:
+ *   y_lo = magnitude * (x_lo * cos - x_hi * sin),  y_hi = magnitude * (x_lo * sin + x_hi * cos)
+ * with (lo, hi) = (2p, 2p+1), or (p, p + n_rot/2) with TCRV_CUDA_ROPE_HALVES; elements n_rot..dim
+ * are copied.  TCRV_CUDA_ROPE_INVERSE turns by the negative angle: the gradient with respect to x,
+ * given that with respect to y.  `positions` is int32, or int64 with TCRV_CUDA_ROPE_POSITIONS_I64.
+ * Up to 4 tensors (queries and keys) share one launch and each token's angles; strides count
+ * elements, the elements of a head are adjacent; y == x with equal strides works in place, any other
+ * overlap does not. */
+#define TCRV_CUDA_ROPE_HALVES 1u
+#define TCRV_CUDA_ROPE_INVERSE 2u
+#define TCRV_CUDA_ROPE_POSITIONS_I64 4u
+typedef struct {
+  const void *x;
+  void *y;
+  size_t heads;
+  size_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+} tcrv_cuda_rope_tensor;
+int tcrv_cuda_rope_rows(int type, size_t tokens, size_t dim, size_t n_rot, const tcrv_cuda_rope_tensor *tensors,
+                        size_t count, const void *positions, const double *freqs, float magnitude, unsigned flags,
+                        tcrv_cuda_stream stream);
+
+/* The angle per position of each pair, freqs[p] for p < n_rot / 2: theta_base^(-2p / n_rot), and for
+ * contexts `factor` times longer than the trained `original` positions
+ *   LINEAR  freq / factor;
+ *   YARN    freq * k + freq / factor * (1 - k): k = 1 up to the pair that turns `high` times within
+ *           `original` positions, 0 from the one that turns `low` times, linear in p between (the two
+ *           ends at whole pairs, rounded outwards);
+ *   BANDS   the same blend with k = (turns - low) / (high - low), clamped to 0..1, where
+ *           turns = original * freq / (2 pi). */
+#define TCRV_CUDA_ROPE_SCALING_NONE 0
+#define TCRV_CUDA_ROPE_SCALING_LINEAR 1
+#define TCRV_CUDA_ROPE_SCALING_YARN 2
+#define TCRV_CUDA_ROPE_SCALING_BANDS 3
+int tcrv_cuda_rope_frequencies_f64(size_t n_rot, double theta_base, int scaling, double factor, double original,
+                                   double low, double high, double *freqs, tcrv_cuda_stream stream);
+
+/* The cache: `pages` pages of 16 * groups tokens.  A page holds, for each kv head and each group of
+ * 16 tokens in turn, 18 * dim bytes (dim a multiple of 32, nb = dim / 32 blocks to a row):
+ *   [0, 8 dim)        key quants:   32-bit word ((half*8 + g)*4 + t)*nb + b = bytes 4t..4t+3 of block b
+ *                     of token g + 8 half
+ *   [8 dim, 16 dim)   value quants: 32-bit word ((half*8 + g)*4 + t)*nb + b = bytes 2g, 2g+1 of block b
+ *                     of token 2t + 8 half, then the same of the token after it
+ *   [16 dim, 17 dim)  key scales:   fp16 [token][b]
+ *   [17 dim, 18 dim)  value scales: fp16 [token][b]
+ * where a block's scale and 16 quant bytes are those of block_q4_0.  Pages are page_stride bytes
+ * apart; `data` and page_stride are multiples of 16.  A token's place is its slot,
+ * page * 16 * groups + token in the page. */
+typedef struct {
+  uint8_t *data;
+  size_t pages, kv_heads, groups, dim, page_stride;
+} tcrv_cuda_kv_cache;
+
+/* Rows of `k` and `v` (element [row][head][d], strides in elements, d adjacent) into the slots
+ * slots[row], quantised as tcrv_cuda_quantize_row_q4_0 does.  A row whose slot is outside the cache
+ * (a padding row: -1) is skipped.  Two rows of one call must not share a slot. */
+int tcrv_cuda_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_stride, size_t k_head_stride,
+                            const void *v, size_t v_row_stride, size_t v_head_stride, const int64_t *slots,
+                            const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream);
+/* The inverse: k[row][head][d] and v (contiguous, d * q rounded to `type`) of the given slots; zeros
+ * for a slot outside the cache. */
+int tcrv_cuda_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *slots,
+                           const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream);
+
+/* A step's book-keeping, for `requests` (at most 16384) requests that hold context_lens[r] tokens and
+ * add new_lens[r]: pages for the new tokens are popped from the free stack (free_pages[*free_count - 1]
+ * first, in the order of requests and then of their pages) into block_table[r * table_stride + i], and
+ *   first_rows[requests + 1]  first row of each request, then the number of rows
+ *   kv_lens[requests]         context_lens + new_lens
+ *   slots[rows]               slot of each row; -1 behind the last one
+ *   positions[rows]           position of each row in its request; 0 behind the last one
+ *   row_requests[rows]        request of each row; -1 behind the last one
+ *   info[4]                   status, rows used, pages taken, pages left in the free stack
+ * If the step is impossible nothing is taken: the status is 1 (too few free pages), 2 (a request needs
+ * more than `width` pages), 3 (more than `rows` rows), 4 (a negative length, or a free count that is
+ * negative or more than free_capacity) - the last one that applies -, first_rows and row counts are 0,
+ * slots are -1, kv_lens are context_lens and the block table stays.  free_count may be info + 3 of an
+ * earlier call, also of this one's info. */
+typedef struct {
+  size_t requests, page_tokens, width, rows, free_capacity;
+  const int32_t *context_lens, *new_lens;
+  int32_t *block_table;
+  size_t table_stride;
+  const int32_t *free_pages, *free_count;
+  int32_t *first_rows, *kv_lens;
+  int64_t *slots;
+  int32_t *positions, *row_requests, *info;
+} tcrv_cuda_kv_plan_call;
+int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream stream);
+
+/* out[row][head] = softmax(scale * q[row][head] . K) V over the cache.  Request r's rows are
+ * first_rows[r] .. first_rows[r+1] - 1 (at most max_new of them; without first_rows: row r alone), the
+ * last tokens of the kv_lens[r] that it has in the pages block_table[r * table_stride ..]; row i of n
+ * sees the tokens up to its own position kv_lens[r] - n + i and, if window > 0, only the last `window`
+ * of those.  heads is a multiple of kv_heads, query heads h * (heads / kv_heads) .. share kv head h.
+ * A row that sees nothing gets zeros and lse = -inf; rows outside every request are left as they were.
+ * Tokens behind `width` pages and tokens in pages outside the cache count as unseen.  `lse` (may be
+ * null) gets the natural logarithm of each row's soft-max sum, [row][head].  Strides count elements,
+ * the elements of a head are adjacent.  dim: 64, 96, 128, 192 or 256.
+ * `workspace` holds the partial results of contexts that are split: 256-byte aligned,
+ * tcrv_cuda_attention_q4_0_workspace_bytes(call) bytes (which ignores the call's pointers); nothing in
+ * it outlives the call, and calls that may run at the same time need one each. */
+typedef struct {
+  int type;
+  size_t requests, rows, heads, max_new;
+  const void *q;
+  size_t q_row_stride, q_head_stride;
+  void *out;
+  size_t out_row_stride, out_head_stride;
+  float *lse;
+  tcrv_cuda_kv_cache cache;
+  const int32_t *block_table;
+  size_t width, table_stride;
+  const int32_t *kv_lens, *first_rows;
+  float scale;
+  size_t window;
+  void *workspace;
+  size_t workspace_bytes;
+} tcrv_cuda_attention_call;
+size_t tcrv_cuda_attention_q4_0_workspace_bytes(const tcrv_cuda_attention_call *call);
+int tcrv_cuda_attention_q4_0(const tcrv_cuda_attention_call *call, tcrv_cuda_stream stream);
+
 /* Debug variant of the integer stage: sumi[(ir*nc + col)*(n/32) + ib], bit-exact int32. */
 int tcrv_cuda_block_sums_q4_0_q8_0(size_t n, int32_t *sumi, const uint8_t *vx, const uint8_t *vy,
                                    size_t by, size_t nr, size_t nc, size_t bx, tcrv_cuda_stream stream);

@@ -62,6 +62,14 @@ ABI = {
     "tcrv_cuda_vec_soft_max_f32": [_sz, _p, _p, ctypes.c_float, _p, _p],
     "tcrv_cuda_rope_cache_f32": [_sz, ctypes.c_float, ctypes.c_float, _p, _p, _p],
     "tcrv_cuda_rope_apply_f32": [_sz, _p, _p, _p, _sz, _sz, _sz, _p],
+    "tcrv_cuda_rope_rows": [_i, _sz, _sz, _sz, _p, _sz, _p, _p, ctypes.c_float, ctypes.c_uint, _p],
+    "tcrv_cuda_rope_frequencies_f64": [_sz, ctypes.c_double, _i, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                       ctypes.c_double, _p, _p],
+    "tcrv_cuda_kv_store_q4_0": [_i, _sz, _p, _sz, _sz, _p, _sz, _sz, _p, _p, _p],
+    "tcrv_cuda_kv_load_q4_0": [_i, _sz, _p, _p, _p, _p, _p],
+    "tcrv_cuda_kv_plan": [_p, _p],
+    "tcrv_cuda_attention_q4_0_workspace_bytes": [_p],
+    "tcrv_cuda_attention_q4_0": [_p, _p],
     "tcrv_cuda_pack_q4_0_to_q4_0x16": [_sz, _p, _p, _p],
     "tcrv_cuda_unpack_q4_0x16_to_q4_0": [_sz, _p, _p, _p],
     "tcrv_cuda_q4_0_q8_0_integer_core": [_p, _p, _p, _p, _p, _sz, _p],
@@ -125,6 +133,7 @@ _RESTYPES = {
     "tcrv_cuda_gemm_workspace_bytes": _sz,
     "tcrv_cuda_repack_gemv_parts": _sz,
     "tcrv_cuda_repack_gemm_workspace_bytes": _sz,
+    "tcrv_cuda_attention_q4_0_workspace_bytes": _sz,
 }
 
 _lib = None
@@ -542,6 +551,118 @@ def rope_cache(n_dims: int, theta_base: float, theta_scale: float, device="cuda"
 def rope_apply(x, cache, out=None):
     """Rotates the rows of a 2-D (rows, n_dims) tensor with one shared angle cache."""
     return _native.rope_apply(x, cache, out)
+
+
+# ------------------------------------------------------------------ attention over a paged Q4_0 cache
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2, "bands": 3}
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+
+
+def rope_frequencies(n_rot: int, theta_base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                     original: float = 0.0, low: float = 1.0, high: float = 32.0, device="cuda"):
+    """Angle per position of each of the n_rot / 2 pairs, a float64 vector for `rope`.
+
+    `scaling` stretches contexts to `factor` times the `original` positions that a model was trained
+    on: "linear" slows every pair, "yarn" and "bands" only those that turn less than `high` times within
+    `original`, fully from `low` turns down (yarn: linear in the pair's index, bands: in its turns)."""
+    import torch
+
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {sorted(ROPE_SCALINGS)}")
+    if n_rot < 0:
+        raise ValueError("n_rot must not be negative")
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        freqs = torch.empty(n_rot // 2, dtype=torch.float64, device=device)
+        _check(lib().tcrv_cuda_rope_frequencies_f64(n_rot, theta_base, ROPE_SCALINGS[scaling], factor, original, low, high,
+                                                    freqs.data_ptr() or None, _stream()), "tcrv_cuda_rope_frequencies_f64")
+    return freqs
+
+
+def rope(x, positions, freqs, halves: bool = False, magnitude: float = 1.0, inverse: bool = False, out=None):
+    """Rotates the first 2 * len(freqs) elements of every head of `x`, (tokens, heads, dim) float32,
+    float16 or bfloat16, by positions[token] * freqs[pair]; pairs are neighbours, or with `halves` the
+    same place of the two halves.  positions: int32 or int64.  `magnitude` multiplies the result.
+    `inverse` turns back: the gradient of x, given that of the result.  out=x works in place."""
+    return _native.rope(x, None, positions, freqs, halves, magnitude, inverse, out, None)
+
+
+def rope_qk(q, k, positions, freqs, halves: bool = False, magnitude: float = 1.0, inverse: bool = False, out=None):
+    """`rope` of queries and keys of the same tokens in one launch; `out` is a pair."""
+    oq, ok = out if out is not None else (None, None)
+    return _native.rope(q, k, positions, freqs, halves, magnitude, inverse, oq, ok)
+
+
+class KvPlan(tuple):
+    """What `kv_plan` gives: CUDA tensors by the names below, in the order of a tuple."""
+
+    __slots__ = ()
+    first_rows = property(lambda self: self[0])
+    kv_lens = property(lambda self: self[1])
+    slots = property(lambda self: self[2])
+    positions = property(lambda self: self[3])
+    requests = property(lambda self: self[4])
+    info = property(lambda self: self[5])
+
+
+def kv_plan(context_lens, new_lens, block_table, free_pages, free_count, page_tokens: int, rows: int, out=None):
+    """Pages, slots and positions of a step in which request r, holding context_lens[r] tokens, adds
+    new_lens[r]; everything stays on the GPU.
+
+    New pages are popped from the end of free_pages[:free_count] into `block_table` (requests, width),
+    which is updated in place.  Returns a KvPlan: first_rows (requests + 1), kv_lens, and for each of
+    `rows` rows slots (-1 behind the last), positions and requests; info = (status, rows used, pages
+    taken, pages left).  A step that cannot be done has a status other than 0, takes nothing and has no
+    rows: 1 too few free pages, 2 more than `width` pages to a request, 3 more than `rows` rows, 4 a
+    negative length or an impossible free count.  All int32 but the slots (int64).  `out`, an earlier
+    plan of the same sizes, is overwritten; `free_count` may be its info[3:4]."""
+    return KvPlan(_native.kv_plan(context_lens, new_lens, block_table, free_pages, free_count, page_tokens, rows, out))
+
+
+def kv_cache_q4_0(pages: int, kv_heads: int, page_tokens: int, dim: int, device="cuda"):
+    """An empty cache: uint8 (pages, kv_heads, page_tokens / 16, 18 * dim), 9/16 byte for each value.
+
+    16 tokens of a head form a group of 18 * dim bytes: key quants, value quants, key scales and value
+    scales, laid out for the tensor cores (tcrv_cuda_kv_cache in include/tcrv_cuda.h); kv_store_q4_0 and
+    kv_load_q4_0 write and read it by slot = page * page_tokens + token in the page."""
+    import torch
+
+    if page_tokens <= 0 or page_tokens % 16 or dim <= 0 or dim % QK:
+        raise ValueError("page_tokens must be a multiple of 16 and dim one of 32")
+    return torch.zeros((pages, kv_heads, page_tokens // 16, 18 * dim), dtype=torch.uint8, device=device)
+
+
+def kv_store_q4_0(cache, k, v, slots):
+    """Quantises the rows of `k` and `v`, (tokens, kv_heads, dim), into the int64 slots of `cache`, by the
+    rule of quantize_q4_0.  A slot outside the cache (-1) skips its row; no slot may come twice."""
+    return _native.kv_store(cache, k, v, slots)
+
+
+def kv_load_q4_0(cache, slots, dtype=None):
+    """(k, v) of the given slots, (len(slots), kv_heads, dim) in `dtype` (float32); zeros for a slot
+    outside the cache."""
+    import torch
+
+    types = {None: TYPE_F32, torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if dtype not in types:
+        raise TypeError("dtype must be float32, float16 or bfloat16")
+    return _native.kv_load(cache, slots, types[dtype])
+
+
+def attention_q4_0(q, cache, block_table, kv_lens, first_rows=None, max_new: int = 1, scale=None, window: int = 0, out=None,
+                   with_lse: bool = False, workspace=None):
+    """softmax(scale * q K^T) V of each query row over its request's pages.
+
+    q: (rows, heads, dim) float32, float16 or bfloat16, heads a multiple of the cache's; dim 64, 96,
+    128, 192 or 256.  Request r has the rows first_rows[r] .. first_rows[r + 1] - 1 (at most max_new; one
+    row each without first_rows), the last tokens of the kv_lens[r] that block_table[r] holds; a row sees
+    the tokens up to its own, with `window` only the last `window` of them.  scale: 1 / sqrt(dim).
+    A row that sees nothing gives zeros (lse -inf); rows outside every request are left as they were.
+    Returns out, or (out, lse) with lse (rows, heads) float32, the natural logarithm of the row's
+    soft-max sum.  `workspace`: a uint8 tensor to use instead of a new one; calls that may overlap on the
+    GPU need one each."""
+    return _native.attention(q, cache, block_table, kv_lens, first_rows, max_new, scale, window, out, with_lse, workspace)
 
 
 # ------------------------------------------------------------------ N-sharding (multi-GPU GEMM)

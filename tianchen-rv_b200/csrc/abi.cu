@@ -623,4 +623,157 @@ int tcrv_cuda_gemm_q4_0_q8_0_static_scratch(size_t n, float *s, const uint8_t *v
   return launch_gemm_static_scratch(n, s, vx, bx, vy, by, nr, nc, bs, as_stream(stream));
 }
 
+// ---- attention over a paged Q4_0 cache
+
+}  // extern "C"
+
+namespace {
+
+bool known_type(int type) { return type == TCRV_CUDA_TYPE_F32 || type == TCRV_CUDA_TYPE_F16 || type == TCRV_CUDA_TYPE_BF16; }
+
+constexpr size_t kManyRows = 0x7fffffff;  // rows, tokens and lengths are 32-bit inside the kernels
+
+int check_kv_cache(const tcrv_cuda_kv_cache &c) {
+  if (c.dim == 0 || c.dim % TCRV_QK != 0 || c.kv_heads == 0 || c.groups == 0)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (c.dim > 1024 || c.kv_heads > 65535 || c.groups > 65535 || c.pages > kManyRows)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (c.pages != 0 && (!c.data || reinterpret_cast<uintptr_t>(c.data) % 16 != 0 || c.page_stride % 16 != 0 ||
+                       (c.pages > 1 && c.page_stride < c.kv_heads * c.groups * 18 * c.dim)))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  return TCRV_CUDA_OK;
+}
+
+int check_attention(const tcrv_cuda_attention_call &c) {
+  const int st = check_kv_cache(c.cache);
+  if (st != TCRV_CUDA_OK)
+    return st;
+  if (!known_type(c.type) || c.heads == 0 || c.heads % c.cache.kv_heads != 0 || (c.requests != 0 && c.max_new == 0))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (c.cache.dim != 64 && c.cache.dim != 96 && c.cache.dim != 128 && c.cache.dim != 192 && c.cache.dim != 256)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (c.heads > 65535 || c.requests > kManyRows || c.rows > kManyRows || c.max_new > kManyRows / c.heads ||
+      c.width > kManyRows / (16 * c.cache.groups))
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  return TCRV_CUDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tcrv_cuda_rope_rows(int type, size_t tokens, size_t dim, size_t n_rot, const tcrv_cuda_rope_tensor *tensors,
+                        size_t count, const void *positions, const double *freqs, float magnitude, unsigned flags,
+                        tcrv_cuda_stream stream) {
+  if (!known_type(type) || n_rot % 2 != 0 || n_rot > dim || count > 4 || (count != 0 && !tensors) ||
+      (flags & ~(TCRV_CUDA_ROPE_HALVES | TCRV_CUDA_ROPE_INVERSE | TCRV_CUDA_ROPE_POSITIONS_I64)) != 0)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (dim > 4096 || tokens > kManyRows)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (tokens == 0 || dim == 0)
+    return TCRV_CUDA_OK;
+  size_t heads = 0;
+  for (size_t j = 0; j < count; ++j) {
+    if (tensors[j].heads == 0)
+      continue;
+    if (!tensors[j].x || !tensors[j].y)
+      return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+    if (tensors[j].heads > 65535)
+      return TCRV_CUDA_ERR_UNSUPPORTED;
+    heads += tensors[j].heads;
+  }
+  if (heads == 0)
+    return TCRV_CUDA_OK;
+  if (!positions || (n_rot != 0 && !freqs))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  return launch_rope_rows(type, tokens, dim, n_rot, tensors, count, positions, freqs, magnitude, flags, as_stream(stream));
+}
+
+int tcrv_cuda_rope_frequencies_f64(size_t n_rot, double theta_base, int scaling, double factor, double original,
+                                   double low, double high, double *freqs, tcrv_cuda_stream stream) {
+  if (n_rot % 2 != 0 || !(theta_base > 1.0) || !(factor > 0.0) || scaling < TCRV_CUDA_ROPE_SCALING_NONE ||
+      scaling > TCRV_CUDA_ROPE_SCALING_BANDS || (n_rot != 0 && !freqs))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (scaling >= TCRV_CUDA_ROPE_SCALING_YARN && (!(original > 0.0) || !(low > 0.0) || !(high > low)))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (n_rot > 4096)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  return launch_rope_frequencies_f64(n_rot, theta_base, scaling, factor, original, low, high, freqs, as_stream(stream));
+}
+
+int tcrv_cuda_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_stride, size_t k_head_stride,
+                            const void *v, size_t v_row_stride, size_t v_head_stride, const int64_t *slots,
+                            const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream) {
+  if (!cache || !known_type(type))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  const int st = check_kv_cache(*cache);
+  if (st != TCRV_CUDA_OK)
+    return st;
+  if (rows == 0)
+    return TCRV_CUDA_OK;
+  if (!k || !v || !slots)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (rows > kManyRows)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  return launch_kv_store_q4_0(type, rows, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, slots, *cache,
+                              as_stream(stream));
+}
+
+int tcrv_cuda_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *slots,
+                           const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream) {
+  if (!cache || !known_type(type))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  const int st = check_kv_cache(*cache);
+  if (st != TCRV_CUDA_OK)
+    return st;
+  if (rows == 0)
+    return TCRV_CUDA_OK;
+  if (!k || !v || !slots || reinterpret_cast<uintptr_t>(k) % 16 != 0 || reinterpret_cast<uintptr_t>(v) % 16 != 0)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (rows > kManyRows)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  return launch_kv_load_q4_0(type, rows, k, v, slots, *cache, as_stream(stream));
+}
+
+int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream stream) {
+  if (!call || call->page_tokens == 0)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  const tcrv_cuda_kv_plan_call &c = *call;
+  if (c.requests > 16384 || c.page_tokens > 65536 || c.rows > kManyRows || c.width > kManyRows / c.page_tokens ||
+      c.free_capacity > kManyRows)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (!c.free_count || !c.first_rows || !c.info || (c.free_capacity != 0 && !c.free_pages) ||
+      (c.requests != 0 && (!c.context_lens || !c.new_lens || !c.kv_lens)) ||
+      (c.requests != 0 && c.width != 0 && !c.block_table) || (c.requests > 1 && c.table_stride < c.width) ||
+      (c.rows != 0 && (!c.slots || !c.positions || !c.row_requests)))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  return launch_kv_plan(c, as_stream(stream));
+}
+
+size_t tcrv_cuda_attention_q4_0_workspace_bytes(const tcrv_cuda_attention_call *call) {
+  if (!call)
+    return 0;
+  tcrv_cuda_attention_call c = *call;
+  c.cache.pages = 0;  // (pointers do not matter here)
+  if (check_attention(c) != TCRV_CUDA_OK || c.requests == 0)
+    return 0;
+  return attention_workspace_bytes(c);
+}
+
+int tcrv_cuda_attention_q4_0(const tcrv_cuda_attention_call *call, tcrv_cuda_stream stream) {
+  if (!call)
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  const tcrv_cuda_attention_call &c = *call;
+  const int st = check_attention(c);
+  if (st != TCRV_CUDA_OK)
+    return st;
+  if (c.requests == 0 || c.rows == 0)
+    return TCRV_CUDA_OK;
+  if (!c.q || !c.out || !c.kv_lens || (c.width != 0 && !c.block_table) || (c.requests > 1 && c.table_stride < c.width))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  if (!c.workspace || reinterpret_cast<uintptr_t>(c.workspace) % 256 != 0 || c.workspace_bytes < attention_workspace_bytes(c))
+    return TCRV_CUDA_ERR_WORKSPACE;
+  return launch_attention_q4_0(c, as_stream(stream));
+}
+
 }  // extern "C"

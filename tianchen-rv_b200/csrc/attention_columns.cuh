@@ -1,0 +1,774 @@
+// Attention of a few query rows per request over the paged Q4_0 cache (decode, drafted tokens, and
+// every call whose rows need more than fp16 products): the context's tokens are the M side of the
+// tensor cores' m16n8k16 product and the query rows its N side,
+//   S^T[token][row] = K q^T        and        O^T[d][row] = V^T P^T,
+// so eight rows fill a tile that the other way round would be half empty, and a key or value operand is
+// used as it lies in the cache (kv_layout.cuh): one AND with a mask turns a word into a register of the
+// operand.
+//
+// Numbers.  A cached value is d * (n - 8).  Its integer part is exact in fp16 and the products with it are
+// summed in f32; the scales stay outside: the key's multiplies the f32 sum over its block, the value's
+// multiplies the soft-max weight, one operand per block.  What is rounded is the query row (scaled by a
+// power of two so that its largest element lies in [2^14, 2^15)) and the weight times the value's scale:
+//   fp16 and bf16 calls: both to one fp16 term, 2^-12 relative (a 16-bit query is exact);
+//   f32 calls: both to two fp16 terms, 2^-22 relative, in neighbouring columns of one tile.  The value
+//   scales are lifted by a power of two that follows the largest one seen, like the running maximum.
+// Maximum, sum and accumulators are f32.
+#pragma once
+
+#include "async_copy.cuh"
+#include "kv_layout.cuh"
+
+namespace tcrv {
+namespace attention {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kUnitGroups = 2;                             // groups of 16 tokens to a warp's step
+constexpr int kUnitTokens = kUnitGroups * kGroupTokens;
+constexpr int kCombineThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ColumnParams {
+  tcrv_cuda_attention_call call;
+  uint32_t group;  // query heads to a kv head
+  DeviceErrorWords errors;
+};
+
+// What the combine step has to know of the context range that begins in CTA c and ends in a later one.
+struct SplitRange {
+  int32_t valid, request, head, column_group, last_cta;
+  int32_t pad[3];
+};
+
+// Workspace: one SplitRange per CTA, then (maximum, sum) and the accumulators of two partial ranges per
+// CTA (the one that began before it, the one that ends after it).
+__host__ __device__ inline size_t column_stats_offset(size_t ctas) { return ctas * sizeof(SplitRange); }
+__host__ __device__ inline size_t column_sums_offset(size_t ctas, size_t rows) {
+  return column_stats_offset(ctas) + 2 * ctas * rows * 2 * sizeof(float);
+}
+inline size_t column_workspace_bytes(size_t ctas, size_t rows, size_t dim) {
+  return column_sums_offset(ctas, rows) + 2 * ctas * rows * dim * sizeof(float);
+}
+
+inline int ctas_per_sm(int nb, int nt) { return nb * nt <= 4 ? 2 : 1; }
+
+template <int NB, int NT, int TERMS>
+struct ColumnLayout {
+  static constexpr int kDim = 32 * NB;
+  static constexpr int kStages = NB * NT <= 2 ? 4 : NB * NT <= 3 ? 3 : NB >= 6 ? 2 : NB * NT > 4 ? 4 : 2;
+  static constexpr int kUnitBytes = kUnitGroups * 18 * kDim;
+  static constexpr int kTileRows = 8 / TERMS;    // query rows of a tile
+  static constexpr int kRows = NT * kTileRows;   // of a column group
+  static constexpr int kSums = kStages * kWarps * kUnitBytes;                     // f32 [warp][row of a tile][d]
+  static constexpr int kQuery = kSums + kWarps * kTileRows * kDim * 4;            // fp16 operand of the rows
+  static constexpr int kStats = kQuery + NT * NB * 512;                           // f32 [warp][row][max, sum]
+  static constexpr int kRowInfo = kStats + kWarps * kRows * 2 * 4;                // f32 scale, int position
+  static constexpr int kFlags = kRowInfo + kRows * 8;                             // u32 [stage][warp]
+  static constexpr int kBars = (kFlags + kStages * kWarps * 4 + 7) / 8 * 8;
+  static constexpr int kBytes = kBars + kStages * kWarps * 8;
+};
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8 x 8 transpose of 16-bit elements held two to a lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) {
+  uint32_t u;
+  memcpy(&u, &h, 4);
+  return u;
+}
+__device__ __forceinline__ __half2 bits_half2(uint32_t u) {
+  __half2 h;
+  memcpy(&h, &u, 4);
+  return h;
+}
+
+// Two nibbles n at bits 0..3 and 16..19 -> the fp16 pair n - 8: OR-ed into 1024.0 they are 1024 + n, and
+// the subtraction is exact.  At bits 4..7 and 20..23 they make 1024 + 16 n: times 1/16, less 72.
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) {
+  const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
+  return half2_bits(__hsub2(bits_half2(u), bits_half2(0x64086408u)));
+}
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) {
+  const uint32_t u = (w & 0x00f000f0u) | 0x64006400u;
+  return half2_bits(__hfma2(bits_half2(u), bits_half2(0x2c002c00u), bits_half2(0xd480d480u)));
+}
+
+// The words of one lane in one half of a group's quants, or one token's scales: N adjacent elements.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t *p) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
+      w[2 * i] = v.x, w[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+  }
+}
+template <int NB>
+__device__ __forceinline__ void load_scales(float (&d)[NB], const uint8_t *p) {
+  if constexpr (NB % 2 == 0) {
+    uint32_t w[NB / 2];
+    load_words<NB / 2>(w, p);
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) {
+      const float2 f = __half22float2(bits_half2(w[i]));
+      d[2 * i] = f.x, d[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      d[i] = __half2float(reinterpret_cast<const __half *>(p)[i]);
+  }
+}
+
+// What a call asks of one request.
+struct Request {
+  int32_t rows, first_row, len, first_unit, units, column_groups;
+};
+
+__device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t r, int group_rows) {
+  const tcrv_cuda_attention_call &c = p.call;
+  Request q;
+  long long first = c.first_rows ? c.first_rows[r] : r, end = c.first_rows ? c.first_rows[r + 1] : r + 1ll;
+  if (first < 0)
+    first = end = 0;
+  if (end > static_cast<long long>(c.rows))
+    end = static_cast<long long>(c.rows);
+  long long rows = end - first;
+  rows = rows < 0 ? 0 : rows > static_cast<long long>(c.max_new) ? static_cast<long long>(c.max_new) : rows;
+  long long len = c.kv_lens[r];
+  const long long most = static_cast<long long>(c.width) * c.cache.groups * kGroupTokens;
+  len = len < 0 ? 0 : len > most ? most : len;
+  q.rows = static_cast<int32_t>(rows);
+  q.first_row = static_cast<int32_t>(first);
+  q.len = static_cast<int32_t>(len);
+  // the first row sees least far back
+  long long low = c.window ? len - rows + 1 - static_cast<long long>(c.window) : 0;
+  low = low < 0 ? 0 : low;
+  q.first_unit = static_cast<int32_t>(low / kUnitTokens);
+  const int32_t units = static_cast<int32_t>((len + kUnitTokens - 1) / kUnitTokens) - q.first_unit;
+  q.units = rows == 0 ? 0 : units < 1 ? 1 : units;  // (a request that sees nothing still writes its zeros)
+  q.column_groups = static_cast<int32_t>((rows * p.group + group_rows - 1) / group_rows);
+  return q;
+}
+
+__device__ __forceinline__ long long request_work(const ColumnParams &p, const Request &q) {
+  return static_cast<long long>(q.units) * q.column_groups * static_cast<long long>(p.call.cache.kv_heads);
+}
+
+// A place in the list of all units: requests, then kv heads, then column groups, then units.
+struct Cursor {
+  uint32_t r;
+  Request q;
+  long long request_begin;  // first unit of the request
+  int32_t segment;          // head * column_groups + column group
+  __device__ __forceinline__ long long begin() const { return request_begin + static_cast<long long>(segment) * q.units; }
+  __device__ __forceinline__ long long end() const { return begin() + q.units; }
+  // moves to the segment that holds unit u, which is not before this one (u is inside the list)
+  __device__ __forceinline__ void seek(const ColumnParams &p, long long u, int group_rows) {
+    while (u >= end()) {
+      const int32_t segments = q.column_groups * static_cast<int32_t>(p.call.cache.kv_heads);
+      if (++segment < segments)
+        continue;
+      request_begin += static_cast<long long>(segments) * q.units;
+      segment = 0;
+      do
+        q = load_request(p, ++r, group_rows);
+      while (q.units == 0);
+    }
+  }
+};
+
+__device__ __forceinline__ long long cta_begin(long long work, int cta, int ctas) { return work * cta / ctas; }
+
+// The list's length and the segment of this CTA's first unit.  Each thread sums a run of requests.
+__device__ __forceinline__ long long find_start(const ColumnParams &p, int group_rows, long long *scratch, Cursor *out) {
+  const uint32_t n = static_cast<uint32_t>(p.call.requests), per = (n + kThreads - 1) / kThreads;
+  const uint32_t r0 = threadIdx.x * per, r1 = min(n, r0 + per);
+  long long mine = 0;
+  for (uint32_t r = r0; r < r1; ++r)
+    mine += request_work(p, load_request(p, r, group_rows));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long s = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, s, off);
+    if (lane >= off)
+      s += o;
+  }
+  if (lane == 31)
+    scratch[warp] = s;
+  __syncthreads();
+  long long before = s - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp)
+      before += scratch[w];
+    total += scratch[w];
+  }
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + kWarps - 1) / kWarps));
+  if (static_cast<int>(blockIdx.x) < ctas) {
+    const long long u = cta_begin(total, blockIdx.x, ctas);
+    if (before <= u && u < before + mine) {
+      Cursor c;
+      for (c.r = r0;; ++c.r) {
+        c.q = load_request(p, c.r, group_rows);
+        const long long w = request_work(p, c.q);
+        if (u < before + w)
+          break;
+        before += w;
+      }
+      c.request_begin = before;
+      c.segment = static_cast<int32_t>((u - before) / c.q.units);
+      *out = c;
+    }
+  }
+  __syncthreads();
+  return total;
+}
+
+// One row's result: O / l, or zeros where nothing was seen; lse in natural units.
+__device__ __forceinline__ void write_row(const tcrv_cuda_attention_call &c, size_t row, size_t head, uint32_t d, float sum,
+                                          float l, float m) {
+  store_typed(c.out, row * c.out_row_stride + head * c.out_head_stride + d, c.type, l > 0.0f || l != l ? sum / l : 0.0f);
+  if (d == 0 && c.lse != nullptr)
+    c.lse[row * c.heads + head] = l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Work split: the list of all units (32 tokens of one kv head and column group) is cut into one range per
+// CTA of equal length, whatever the contexts' lengths; inside a range the warps take units in turn, each
+// with a ring of its own that its first two lanes fill by bulk copies ahead of use, across segment ends.  A
+// segment that lies in one range is finished there; of one that does not, each CTA leaves maximum, sum and
+// accumulators in the workspace for the combine kernel.  Bound by bytes at decode (9/16 byte a value, used
+// for at most 8 NT columns), with the instructions that unpack them next: about 500 for a warp's unit.
+template <int NB, int NT, int TERMS>
+__global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(const __grid_constant__ ColumnParams p) {
+  using L = ColumnLayout<NB, NT, TERMS>;
+  constexpr int kDim = L::kDim, kStages = L::kStages, kGroupBytes = 18 * kDim, kRows = L::kRows, kTileRows = L::kTileRows;
+  constexpr int kMine = 2 / TERMS;  // query rows of a tile that a lane's two columns belong to
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long scratch[kWarps];
+  __shared__ Cursor start;
+  const tcrv_cuda_attention_call &c = p.call;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t *ring = smem + warp * kStages * L::kUnitBytes;
+  float *sums = reinterpret_cast<float *>(smem + L::kSums);
+  float *stats = reinterpret_cast<float *>(smem + L::kStats);
+  float *row_scale = reinterpret_cast<float *>(smem + L::kRowInfo);
+  int32_t *row_position = reinterpret_cast<int32_t *>(smem + L::kRowInfo) + kRows;
+  volatile uint32_t *flags = reinterpret_cast<volatile uint32_t *>(smem + L::kFlags) + warp * kStages;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * kStages;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s)
+      mbar_init(&bars[s], 1);
+    mbar_fence_init();
+  }
+  pdl_enter();
+  const long long work = find_start(p, kRows, scratch, &start);
+  SplitRange *ranges = static_cast<SplitRange *>(c.workspace);
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (work + kWarps - 1) / kWarps));
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    if (threadIdx.x == 0)
+      ranges[blockIdx.x].valid = 0;
+    return;
+  }
+  const long long u0 = cta_begin(work, blockIdx.x, ctas), u1 = cta_begin(work, blockIdx.x + 1, ctas);
+
+  // ---- this warp's copies: units u0 + warp, u0 + warp + kWarps, ...  Lanes 0 and 1 copy a group each; the
+  // page of the unit to come is read one step before its copy, so that the copy never waits for the table.
+  Cursor ahead = start;
+  long long next = u0 + warp;  // unit whose pages are in `page`
+  const uint8_t *source = nullptr;
+  auto fetch_page = [&]() {
+    source = nullptr;
+    if (next >= u1)
+      return;
+    ahead.seek(p, next, kRows);
+    if (lane < kUnitGroups) {
+      const int64_t group = static_cast<int64_t>(ahead.q.first_unit + (next - ahead.begin())) * kUnitGroups + lane;
+      if (group * kGroupTokens < ahead.q.len) {
+        const uint32_t at = static_cast<uint32_t>(group / static_cast<uint32_t>(c.cache.groups));
+        const uint32_t in_page = static_cast<uint32_t>(group) - at * static_cast<uint32_t>(c.cache.groups);
+        const int32_t page = c.block_table[ahead.r * c.table_stride + at];
+        const uint32_t head = ahead.segment / ahead.q.column_groups;
+        if (page >= 0 && static_cast<size_t>(page) < c.cache.pages)
+          source = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
+                   (static_cast<size_t>(head) * c.cache.groups + in_page) * kGroupBytes;
+      }
+    }
+  };
+  auto issue = [&](int stage) {
+    if (next < u1) {
+      const uint32_t there = __ballot_sync(0xffffffffu, source != nullptr) & 3u;
+      if (lane == 0) {
+        flags[stage] = there;
+        mbar_arrive_expect_tx(&bars[stage], __popc(there) * kGroupBytes);
+      }
+      __syncwarp();
+      if (source != nullptr)
+        bulk_copy_g2s(ring + stage * L::kUnitBytes + lane * kGroupBytes, source, kGroupBytes, &bars[stage]);
+    }
+    next += kWarps;
+    fetch_page();
+  };
+  fetch_page();
+#pragma unroll 1
+  for (int s = 0; s < kStages; ++s)
+    issue(s);
+  int stage = 0;
+  uint32_t parity = 0;
+  bool failed = false;
+
+  Cursor at = start;
+  long long u = u0 + warp;
+  for (long long from = u0; from < u1;) {
+    at.seek(p, from, kRows);
+    const long long seg_begin = at.begin(), seg_end = at.end(), to = seg_end < u1 ? seg_end : u1;
+    const int32_t head = at.segment / at.q.column_groups, column_group = at.segment - head * at.q.column_groups;
+    const int32_t pair0 = column_group * kRows, pairs = min(kRows, at.q.rows * static_cast<int32_t>(p.group) - pair0);
+
+    // ---- the rows' operand: row `i` by warp i % kWarps
+    for (int i = warp; i < kRows; i += kWarps) {
+      float x[NB];
+      float top = 0.0f;
+      const int32_t pair = pair0 + i, token = pair / static_cast<int32_t>(p.group);
+      const int32_t q_head = head * static_cast<int32_t>(p.group) + (pair - token * static_cast<int32_t>(p.group));
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        x[b] = 0.0f;
+        if (i < pairs)
+          x[b] = load_typed(c.q, static_cast<size_t>(at.q.first_row + token) * c.q_row_stride +
+                                     static_cast<size_t>(q_head) * c.q_head_stride + b * 32 + lane, c.type);
+        top = fmaxf(top, fabsf(x[b]));
+      }
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      // 2^k lifts the largest element into [2^14, 2^15); a row of zeros, or one with an infinity, stays
+      int k = 0;
+      if (top > 0.0f && top < INFINITY)
+        k = min(120, 14 - ilogbf(top));
+      const float lift = exp2f(static_cast<float>(k));
+      const int e = lane & 31, kstep = e >> 4, f = e & 15;
+      const int tile = i / kTileRows, n = (i - tile * kTileRows) * TERMS;
+      __half *operand = reinterpret_cast<__half *>(smem + L::kQuery);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const float v = x[b] * lift;
+        const __half hi = __float2half_rn(v);
+        const int place = (((tile * NB + b) * 32 + n * 4 + (f >> 2)) * 4 + kstep * 2 + (f & 1)) * 2 + ((f & 2) >> 1);
+        operand[place] = hi;
+        if constexpr (TERMS == 2)  // the column after it: lanes 4 further on
+          operand[place + 4 * 8] = isfinite(v) ? __float2half_rn(v - __half2float(hi)) : __float2half_rn(0.0f);
+      }
+      if (lane == 0) {
+        row_scale[i] = c.scale * kLog2e * exp2f(static_cast<float>(-k));
+        row_position[i] = i < pairs ? at.q.len - at.q.rows + token : -1;
+      }
+    }
+    __syncthreads();
+    float scale[NT][kMine];
+    int32_t position[NT][kMine];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
+        scale[j][i] = row_scale[row];
+        position[j][i] = row_position[row];
+      }
+    // tokens that every row of the group sees (rows are in order of position)
+    const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
+    const int32_t seen_to = row_position[0], seen_from = window ? row_position[pairs - 1] - window + 1 : 0;
+
+    float m[NT][kMine], l[NT][kMine], o[2 * NB][NT][4];
+    int lifted = -100;  // exponent of the largest value scale so far; the accumulators hold O * 2^(14 - lifted)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        m[j][i] = -INFINITY, l[j][i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[i][j][e] = 0.0f;
+
+    for (; u < to; u += kWarps) {
+      if (!failed && !mbar_wait_bounded(&bars[stage], parity)) {
+        failed = true;
+        raise_device_error(p.errors, kDevErrBarrierTimeout);
+      }
+      const uint8_t *unit = ring + stage * L::kUnitBytes;
+      const uint32_t there = flags[stage];
+      const int32_t token0 = static_cast<int32_t>(at.q.first_unit + (u - seg_begin)) * kUnitTokens;
+
+      // ---- S^T = K q^T
+      float s[kUnitGroups][NT][4];
+#pragma unroll
+      for (int gr = 0; gr < kUnitGroups; ++gr) {
+        const uint8_t *group = unit + gr * kGroupBytes;
+        uint32_t w0[NB], w1[NB];
+        float d0[NB], d1[NB];
+        load_words<NB>(w0, group + lane * NB * 4);
+        load_words<NB>(w1, group + 128 * NB + lane * NB * 4);
+        load_scales<NB>(d0, group + 512 * NB + g * NB * 2);
+        load_scales<NB>(d1, group + 512 * NB + (g + 8) * NB * 2);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[gr][j][e] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t a0[4] = {low_nibbles(w0[b]), low_nibbles(w1[b]), low_nibbles(w0[b] >> 8), low_nibbles(w1[b] >> 8)};
+          const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w1[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b] >> 8)};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(smem + L::kQuery + ((j * NB + b) * 32 + lane) * 16);
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma16816(acc, a0, q.x, q.y);
+            mma16816(acc, a1, q.z, q.w);
+            s[gr][j][0] = fmaf(acc[0], d0[b], s[gr][j][0]);
+            s[gr][j][1] = fmaf(acc[1], d0[b], s[gr][j][1]);
+            s[gr][j][2] = fmaf(acc[2], d1[b], s[gr][j][2]);
+            s[gr][j][3] = fmaf(acc[3], d1[b], s[gr][j][3]);
+          }
+        }
+      }
+
+      // ---- scores in powers of two, the mask, the running maximum and sum
+      const bool whole = there == 3u && token0 >= seen_from && token0 + kUnitTokens - 1 <= seen_to;
+      float pr[kUnitGroups][NT][2][kMine];  // [group][tile][token g or g + 8][row]
+      bool moved = false;
+      float alpha[NT][kMine];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float v = TERMS == 1 ? s[gr][j][2 * h + i] : s[gr][j][2 * h] + s[gr][j][2 * h + 1];
+              v *= scale[j][i];
+              if (!whole) {
+                const int32_t token = token0 + gr * kGroupTokens + h * 8 + g;
+                if (!((there >> gr) & 1u) || token > position[j][i] || (window && token <= position[j][i] - window))
+                  v = -INFINITY;
+              }
+              pr[gr][j][h][i] = v;
+              top = fmaxf(top, v);
+            }
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float now = fmaxf(m[j][i], top), base = now == -INFINITY ? 0.0f : now;
+          alpha[j][i] = exp2_fast(m[j][i] - base);
+          moved |= now != m[j][i];
+          m[j][i] = now;
+          float sum = 0.0f;
+#pragma unroll
+          for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              pr[gr][j][h][i] = exp2_fast(pr[gr][j][h][i] - base);
+              sum += pr[gr][j][h][i];
+            }
+          l[j][i] = fmaf(l[j][i], alpha[j][i], sum);
+        }
+
+      // ---- value scales of this lane's tokens; those of unseen tokens may be anything and count as zero
+      float vd[kUnitGroups][2][NB];
+#pragma unroll
+      for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          load_scales<NB>(vd[gr][h], unit + gr * kGroupBytes + 544 * NB + (g + 8 * h) * NB * 2);
+          if (!whole) {
+            const bool there_is = ((there >> gr) & 1u) && token0 + gr * kGroupTokens + h * 8 + g < at.q.len;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              vd[gr][h][b] = there_is ? vd[gr][h][b] : 0.0f;
+          }
+        }
+      float lift = 1.0f, relift = 1.0f;
+      if constexpr (TERMS == 2) {
+        const auto largest = [&](bool finite_only) {
+          float top = 0.0f;
+#pragma unroll
+          for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                const float d = fabsf(vd[gr][h][b]);
+                top = fmaxf(top, finite_only && d == INFINITY ? 0.0f : d);
+              }
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          return top;
+        };
+        float top = largest(false);
+        if (top == INFINITY)  // (of a token that some rows may not see: their lift goes by the others)
+          top = largest(true);
+        // exponent of an fp16 number, -100 for zero
+        const int e = top > 0.0f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 : -100;
+        if (e > lifted) {
+          relift = exp2f(static_cast<float>(lifted - e));
+          lifted = e;
+          moved = true;
+        }
+        lift = lifted > -100 ? exp2f(static_cast<float>(14 - lifted)) : 1.0f;
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const float f0 = alpha[j][0] * relift, f1 = alpha[j][kMine - 1] * relift;
+            o[i][j][0] *= f0;
+            o[i][j][1] *= f1;
+            o[i][j][2] *= f0;
+            o[i][j][3] *= f1;
+          }
+      }
+
+      // ---- O^T += V^T P^T, the weights times the value scales block by block
+#pragma unroll
+      for (int gr = 0; gr < kUnitGroups; ++gr) {
+        const uint8_t *group = unit + gr * kGroupBytes + 256 * NB;
+        uint32_t w0[NB], w1[NB];
+        load_words<NB>(w0, group + lane * NB * 4);
+        load_words<NB>(w1, group + 128 * NB + lane * NB * 4);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t a0[4] = {low_nibbles(w0[b]), low_nibbles(w0[b] >> 8), low_nibbles(w1[b]), low_nibbles(w1[b] >> 8)};
+          const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b]), high_nibbles(w1[b] >> 8)};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            uint32_t bits[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x0, x1;
+              if constexpr (TERMS == 1) {
+                x0 = pr[gr][j][h][0] * vd[gr][h][b];
+                x1 = pr[gr][j][h][1] * vd[gr][h][b];
+                if (!whole) {  // a weight of zero stays zero, whatever the scale
+                  x0 = pr[gr][j][h][0] == 0.0f ? 0.0f : x0;
+                  x1 = pr[gr][j][h][1] == 0.0f ? 0.0f : x1;
+                }
+              } else {
+                float v = pr[gr][j][h][0] * (vd[gr][h][b] * lift);
+                if (!whole)
+                  v = pr[gr][j][h][0] == 0.0f ? 0.0f : v;
+                x0 = __half2float(__float2half_rn(v));
+                x1 = v - x0;
+              }
+              bits[h] = transpose8x8(half2_bits(__floats2half2_rn(x0, x1)));
+            }
+            mma16816(o[2 * b][j], a0, bits[0], bits[1]);
+            mma16816(o[2 * b + 1][j], a1, bits[0], bits[1]);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      issue(stage);
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+    }
+
+    // ---- the warps' parts of the segment become one
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1)
+          l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], off);
+        if (g == 0) {
+          const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
+          stats[(warp * kRows + row) * 2] = m[j][i];
+          stats[(warp * kRows + row) * 2 + 1] = l[j][i];
+        }
+      }
+    __syncthreads();
+    const bool first = seg_begin < u0, split = first || seg_end > u1;
+    const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
+    uint8_t *ws = static_cast<uint8_t *>(c.workspace);
+    float *part_stats = reinterpret_cast<float *>(ws + column_stats_offset(gridDim.x)) + slot * kRows * 2;
+    float *part_sums = reinterpret_cast<float *>(ws + column_sums_offset(gridDim.x, kRows)) + slot * kRows * kDim;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      // this warp's accumulators on the CTA's maximum
+      float f[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          top = fmaxf(top, stats[(w * kRows + row) * 2]);
+        f[i] = m[j][i] == -INFINITY ? 0.0f : exp2_fast(m[j][i] - top);
+        if constexpr (TERMS == 2)
+          f[i] *= lifted > -100 ? exp2f(static_cast<float>(lifted - 14)) : 1.0f;
+      }
+      float *mine = sums + warp * kTileRows * kDim;
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) {
+        const int d = (i >> 1) * 32 + (i & 1) * 16 + 2 * g;
+        if constexpr (TERMS == 1) {
+          *reinterpret_cast<float2 *>(mine + 2 * t * kDim + d) = make_float2(o[i][j][0] * f[0], o[i][j][2] * f[0]);
+          *reinterpret_cast<float2 *>(mine + (2 * t + 1) * kDim + d) = make_float2(o[i][j][1] * f[1], o[i][j][3] * f[1]);
+        } else {
+          *reinterpret_cast<float2 *>(mine + t * kDim + d) =
+              make_float2((o[i][j][0] + o[i][j][1]) * f[0], (o[i][j][2] + o[i][j][3]) * f[0]);
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < kTileRows * kDim; i += kThreads) {
+        const int row = j * kTileRows + i / kDim, d = i % kDim;
+        if (row >= pairs)
+          break;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          sum += sums[w * kTileRows * kDim + i];
+        if (split)
+          part_sums[row * kDim + d] = sum;
+        if (!split || d == 0) {
+          float top = -INFINITY, total = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w)
+            top = fmaxf(top, stats[(w * kRows + row) * 2]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float mw = stats[(w * kRows + row) * 2];
+            total += mw == -INFINITY ? 0.0f : exp2_fast(mw - top) * stats[(w * kRows + row) * 2 + 1];
+          }
+          if (split) {
+            part_stats[row * 2] = top;
+            part_stats[row * 2 + 1] = total;
+          } else {
+            const int32_t pair = pair0 + row, token = pair / static_cast<int32_t>(p.group);
+            write_row(c, at.q.first_row + token, head * p.group + (pair - token * p.group), d, sum, total, top);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0 && to == u1) {
+      SplitRange range = {};
+      range.valid = !first && seg_end > u1;
+      range.request = static_cast<int32_t>(at.r);
+      range.head = head;
+      range.column_group = column_group;
+      if (range.valid) {  // the CTA that holds the segment's last unit
+        int last = static_cast<int>((seg_end - 1) * ctas / work);
+        while (last + 1 < ctas && cta_begin(work, last + 1, ctas) < seg_end)
+          ++last;
+        while (cta_begin(work, last, ctas) >= seg_end)
+          --last;
+        range.last_cta = last;
+      }
+      ranges[blockIdx.x] = range;
+    }
+    from = to;
+  }
+}
+
+// Joins the parts of a segment that several CTAs hold: block (c, y) does rows y, y + gridDim.y, ... of the segment
+// that begins in CTA c and ends in a later one.
+template <int NB>
+__global__ void __launch_bounds__(kCombineThreads) columns_combine_kernel(const __grid_constant__ ColumnParams p, int rows) {
+  constexpr int kDim = 32 * NB;
+  __shared__ float reduce[2 * kCombineThreads / 32];
+  pdl_enter();
+  const tcrv_cuda_attention_call &c = p.call;
+  const uint8_t *ws = static_cast<const uint8_t *>(c.workspace);
+  const SplitRange range = static_cast<const SplitRange *>(c.workspace)[blockIdx.x];
+  if (!range.valid)
+    return;
+  const Request q = load_request(p, range.request, rows);
+  const float *stats = reinterpret_cast<const float *>(ws + column_stats_offset(gridDim.x));
+  const float *sums = reinterpret_cast<const float *>(ws + column_sums_offset(gridDim.x, rows));
+  const int32_t pair0 = range.column_group * rows, pairs = min(rows, q.rows * static_cast<int32_t>(p.group) - pair0);
+  const int parts = range.last_cta - static_cast<int>(blockIdx.x) + 1;
+  // part i: the second slot of the first CTA, the first slots of the others
+  auto slot = [&](int i) { return 2 * static_cast<size_t>(blockIdx.x + i) + (i == 0 ? 1 : 0); };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int row = blockIdx.y; row < pairs; row += gridDim.y) {
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += kCombineThreads)
+      top = fmaxf(top, stats[(slot(i) * rows + row) * 2]);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (lane == 0)
+      reduce[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kCombineThreads / 32; ++w)
+      top = fmaxf(top, reduce[w]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum[(kDim + kCombineThreads - 1) / kCombineThreads] = {};
+    float total = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float2 ml = *reinterpret_cast<const float2 *>(stats + (slot(i) * rows + row) * 2);
+      const float f = exp2_fast(ml.x - base);
+      total = fmaf(f, ml.y, total);
+#pragma unroll
+      for (int k = 0; k * kCombineThreads < kDim; ++k) {
+        const int d = threadIdx.x + k * kCombineThreads;
+        if (d < kDim)
+          sum[k] = fmaf(f, sums[(slot(i) * rows + row) * kDim + d], sum[k]);
+      }
+    }
+    const int32_t pair = pair0 + row, token = pair / static_cast<int32_t>(p.group);
+#pragma unroll
+    for (int k = 0; k * kCombineThreads < kDim; ++k) {
+      const int d = threadIdx.x + k * kCombineThreads;
+      if (d < kDim)
+        write_row(c, q.first_row + token, range.head * p.group + (pair - token * p.group), d, sum[k], total, top);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace attention
+}  // namespace tcrv

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "tcrv_cuda.h"
+
 namespace tcrv {
 
 int launch_add_f32(const float *lhs, const float *rhs, float *out, size_t n, cudaStream_t stream);
@@ -40,6 +42,20 @@ int launch_dequantize_row_q8_0(const uint8_t *vx, float *y, size_t n, cudaStream
 int launch_dequantize_row_q4_0(const uint8_t *vx, float *y, size_t n, cudaStream_t stream);
 int launch_quantize_row_q8_0(size_t n, const float *x, uint8_t *vy, cudaStream_t stream);
 int launch_quantize_row_q4_0(size_t n, const float *x, uint8_t *vx, cudaStream_t stream);
+
+// rotary positions (rope.cu), the paged Q4_0 cache (kv_cache.cu) and attention over it (attention.cu)
+int launch_rope_rows(int type, size_t tokens, size_t dim, size_t n_rot, const tcrv_cuda_rope_tensor *tensors, size_t count,
+                     const void *positions, const double *freqs, float magnitude, unsigned flags, cudaStream_t stream);
+int launch_rope_frequencies_f64(size_t n_rot, double theta_base, int scaling, double factor, double original, double low,
+                                double high, double *freqs, cudaStream_t stream);
+int launch_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_stride, size_t k_head_stride, const void *v,
+                         size_t v_row_stride, size_t v_head_stride, const int64_t *slots, const tcrv_cuda_kv_cache &cache,
+                         cudaStream_t stream);
+int launch_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *slots, const tcrv_cuda_kv_cache &cache,
+                        cudaStream_t stream);
+int launch_kv_plan(const tcrv_cuda_kv_plan_call &call, cudaStream_t stream);
+size_t attention_workspace_bytes(const tcrv_cuda_attention_call &call);
+int launch_attention_q4_0(const tcrv_cuda_attention_call &call, cudaStream_t stream);
 
 template <bool kQ8W>
 int launch_gemv(size_t n, float *s, const uint8_t *vx, const uint8_t *vy, size_t by, size_t nr, size_t nc,

@@ -9,9 +9,13 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <utility>
 
 #include "tcrv_cuda.h"
 
@@ -507,6 +511,336 @@ TCRV_CALL(repack_gemv, 6) {
   return out.result();
 }
 
+// ---- attention over a paged Q4_0 cache.  These calls run on their operands' device, whichever device is
+// current, and refuse operands on several.
+
+inline int activation_type(const at::Tensor &t) {
+  switch (t.scalar_type()) {
+    case at::kFloat:
+      return TCRV_CUDA_TYPE_F32;
+    case at::kHalf:
+      return TCRV_CUDA_TYPE_F16;
+    case at::kBFloat16:
+      return TCRV_CUDA_TYPE_BF16;
+    default:
+      fail(PyExc_TypeError, "activations must be float32, float16 or bfloat16");
+  }
+}
+
+// A (tokens, heads, dim) tensor whose heads lie in one piece.
+inline const at::Tensor &head_rows(PyObject *o, const char *text) {
+  const at::Tensor &t = tensor(o);
+  if (t.dim() != 3 || (t.size(2) > 1 && t.stride(2) != 1))
+    fail(PyExc_ValueError, text);
+  return t;
+}
+
+// The same as an output: its type and shape, and no element in two places.
+inline const at::Tensor &head_output(PyObject *o, const at::Tensor &like, int64_t rows, int64_t heads, int64_t dim) {
+  const at::Tensor &t = head_rows(o, "an output is (tokens, heads, dim) with adjacent elements of a head");
+  if (t.scalar_type() != like.scalar_type())
+    fail(PyExc_TypeError, "an output has its input's type");
+  if (t.size(0) != rows || t.size(1) != heads || t.size(2) != dim)
+    fail(PyExc_ValueError, "an output has its input's shape");
+  int64_t n[2] = {rows, heads}, st[2] = {t.stride(0), t.stride(1)};
+  if (n[0] <= 1 || (n[1] > 1 && st[1] > st[0])) {  // the closer one first
+    std::swap(n[0], n[1]);
+    std::swap(st[0], st[1]);
+  }
+  if ((n[1] > 1 && st[1] < dim) || (n[0] > 1 && st[0] < (n[1] > 1 ? (n[1] - 1) * st[1] : 0) + dim))
+    fail(PyExc_ValueError, "an output's heads overlap");
+  return t;
+}
+
+inline void same_device(const at::Tensor &a, const at::Tensor &b) {
+  if (a.device() != b.device())
+    fail(PyExc_ValueError, "operands are on different devices");
+}
+
+inline const at::Tensor &dense_beside(PyObject *o, at::ScalarType type, const at::Tensor &like) {
+  const at::Tensor &t = tensor(o);
+  if (t.scalar_type() != type) {
+    PyErr_Format(PyExc_TypeError, "expected dtype torch.%s, got %s", type == at::kInt ? "int32" : type == at::kLong ? "int64" : "float64",
+                 c10::toString(t.scalar_type()));
+    throw PyError{};
+  }
+  if (t.dim() != 1 || !t.is_contiguous())
+    fail(PyExc_ValueError, "lengths, slots, positions and frequencies are contiguous vectors");
+  same_device(t, like);
+  return t;
+}
+
+inline const int32_t *ints(const at::Tensor &t) { return static_cast<const int32_t *>(t.data_ptr()); }
+
+PyObject *pair_of(at::Tensor a, at::Tensor b) {
+  PyObject *x = THPVariable_Wrap(std::move(a)), *y = THPVariable_Wrap(std::move(b));
+  PyObject *r = x != nullptr && y != nullptr ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  if (r == nullptr)
+    throw PyError{};
+  return r;
+}
+
+// rope(q, k or None, positions, freqs, halves, magnitude, inverse, out_q, out_k)
+TCRV_CALL(rope, 9) {
+  const char *text = "x must be (tokens, heads, dim) with adjacent elements of a head";
+  const at::Tensor &q = head_rows(a[0], text);
+  const bool two = a[1] != Py_None;
+  const at::Tensor &k = two ? head_rows(a[1], text) : q;
+  const int type = activation_type(q);
+  if (k.scalar_type() != q.scalar_type())
+    fail(PyExc_TypeError, "queries and keys differ in type");
+  if (k.size(0) != q.size(0) || k.size(2) != q.size(2))
+    fail(PyExc_ValueError, "queries and keys differ in tokens or head size");
+  same_device(q, k);
+  const at::Tensor &any = tensor(a[2]);
+  const bool wide = any.scalar_type() == at::kLong;
+  const at::Tensor &positions = dense_beside(a[2], wide ? at::kLong : at::kInt, q);
+  const at::Tensor &freqs = dense_beside(a[3], at::kDouble, q);
+  if (positions.numel() != q.size(0))
+    fail(PyExc_ValueError, "one position for each token");
+  if (2 * freqs.numel() > q.size(2))
+    fail(PyExc_ValueError, "more frequencies than pairs in a head");
+  const unsigned flags = (truth(a[4]) ? TCRV_CUDA_ROPE_HALVES : 0u) | (truth(a[6]) ? TCRV_CUDA_ROPE_INVERSE : 0u) |
+                         (wide ? TCRV_CUDA_ROPE_POSITIONS_I64 : 0u);
+  const float magnitude = static_cast<float>(real(a[5]));
+  at::Tensor oq, ok;
+  if (a[7] != Py_None)
+    same_device(q, oq = head_output(a[7], q, q.size(0), q.size(1), q.size(2)));
+  if (two && a[8] != Py_None)
+    same_device(q, ok = head_output(a[8], k, k.size(0), k.size(1), k.size(2)));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const cudaStream_t st = stream();
+  check(module, unlocked([&] {
+          if (!oq.defined())
+            oq = empty(q.sizes(), q.scalar_type(), q);
+          if (two && !ok.defined())
+            ok = empty(k.sizes(), k.scalar_type(), k);
+          const auto describe = [](const at::Tensor &x, const at::Tensor &y) {
+            return tcrv_cuda_rope_tensor{x.data_ptr(), y.data_ptr(), static_cast<size_t>(x.size(1)), static_cast<size_t>(x.stride(0)),
+                                         static_cast<size_t>(x.stride(1)), static_cast<size_t>(y.stride(0)), static_cast<size_t>(y.stride(1))};
+          };
+          tcrv_cuda_rope_tensor t[2] = {describe(q, oq), {}};
+          if (two)
+            t[1] = describe(k, ok);
+          return tcrv_cuda_rope_rows(type, static_cast<size_t>(q.size(0)), static_cast<size_t>(q.size(2)),
+                                     static_cast<size_t>(2 * freqs.numel()), t, two ? 2 : 1, positions.data_ptr(),
+                                     static_cast<const double *>(freqs.data_ptr()), magnitude, flags, st);
+        }),
+        "tcrv_cuda_rope_rows");
+  return two ? pair_of(std::move(oq), std::move(ok)) : THPVariable_Wrap(std::move(oq));
+}
+
+// kv_plan(context_lens, new_lens, block_table, free_pages, free_count, page_tokens, rows, six outputs or None)
+TCRV_CALL(kv_plan, 8) {
+  const at::Tensor &table = tensor(a[2]);
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1) ||
+      (table.size(0) > 1 && table.stride(0) < table.size(1)))
+    fail(PyExc_ValueError, "the block table is an int32 (requests, pages) matrix with adjacent pages");
+  const at::Tensor &context = dense_beside(a[0], at::kInt, table), &added = dense_beside(a[1], at::kInt, table);
+  const at::Tensor &free_pages = dense_beside(a[3], at::kInt, table), &free_count = dense_beside(a[4], at::kInt, table);
+  const int64_t n = table.size(0), page = integer(a[5]), rows = integer(a[6]);
+  if (context.numel() != n || added.numel() != n || free_count.numel() != 1)
+    fail(PyExc_ValueError, "one length for each request, and one free count");
+  if (page <= 0 || rows < 0)
+    fail(PyExc_ValueError, "page_tokens must be positive and rows not negative");
+  const int64_t sizes[6] = {n + 1, n, rows, rows, rows, 4};
+  const at::ScalarType types[6] = {at::kInt, at::kInt, at::kLong, at::kInt, at::kInt, at::kInt};
+  at::Tensor out[6];
+  if (a[7] != Py_None) {
+    if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 6)
+      fail(PyExc_TypeError, "out is an earlier plan");
+    for (int i = 0; i < 6; ++i) {
+      out[i] = dense_beside(PyTuple_GET_ITEM(a[7], i), types[i], table);
+      if (out[i].numel() != sizes[i])
+        fail(PyExc_ValueError, "out is a plan of other sizes");
+    }
+  }
+  const c10::cuda::CUDAGuard guard(table.device());
+  const cudaStream_t st = stream();
+  check(module, unlocked([&] {
+          for (int i = 0; i < 6; ++i)
+            if (!out[i].defined())
+              out[i] = empty({sizes[i]}, types[i], table);
+          tcrv_cuda_kv_plan_call c = {};
+          c.requests = static_cast<size_t>(n);
+          c.page_tokens = static_cast<size_t>(page);
+          c.width = static_cast<size_t>(table.size(1));
+          c.rows = static_cast<size_t>(rows);
+          c.free_capacity = static_cast<size_t>(free_pages.numel());
+          c.context_lens = ints(context);
+          c.new_lens = ints(added);
+          c.block_table = static_cast<int32_t *>(table.data_ptr());
+          c.table_stride = static_cast<size_t>(n > 1 ? table.stride(0) : table.size(1));
+          c.free_pages = ints(free_pages);
+          c.free_count = ints(free_count);
+          c.first_rows = static_cast<int32_t *>(out[0].data_ptr());
+          c.kv_lens = static_cast<int32_t *>(out[1].data_ptr());
+          c.slots = static_cast<int64_t *>(out[2].data_ptr());
+          c.positions = static_cast<int32_t *>(out[3].data_ptr());
+          c.row_requests = static_cast<int32_t *>(out[4].data_ptr());
+          c.info = static_cast<int32_t *>(out[5].data_ptr());
+          return tcrv_cuda_kv_plan(&c, st);
+        }),
+        "tcrv_cuda_kv_plan");
+  PyObject *r = PyTuple_New(6);
+  if (r == nullptr)
+    throw PyError{};
+  for (int i = 0; i < 6; ++i) {
+    PyObject *o = THPVariable_Wrap(std::move(out[i]));
+    if (o == nullptr) {
+      Py_DECREF(r);
+      throw PyError{};
+    }
+    PyTuple_SET_ITEM(r, i, o);
+  }
+  return r;
+}
+
+// The cache tensor (pages, kv heads, groups, 18 * dim); pages may lie apart.
+inline tcrv_cuda_kv_cache kv_cache(const at::Tensor &t) {
+  if (t.scalar_type() != at::kByte || t.dim() != 4)
+    fail(PyExc_ValueError, "the cache is a uint8 (pages, kv_heads, groups, 18 * dim) tensor");
+  const int64_t heads = t.size(1), groups = t.size(2), bytes_of = t.size(3);
+  if (heads == 0 || groups == 0 || bytes_of == 0 || bytes_of % (18 * kQK) != 0)
+    fail(PyExc_ValueError, "a group of the cache is 18 * dim bytes, dim a multiple of 32");
+  if (t.stride(3) != 1 || (groups > 1 && t.stride(2) != bytes_of) || (heads > 1 && t.stride(1) != groups * bytes_of))
+    fail(PyExc_ValueError, "a page of the cache must be contiguous");
+  tcrv_cuda_kv_cache c = {};
+  c.pages = static_cast<size_t>(t.size(0));
+  c.kv_heads = static_cast<size_t>(heads);
+  c.groups = static_cast<size_t>(groups);
+  c.dim = static_cast<size_t>(bytes_of / 18);
+  c.page_stride = static_cast<size_t>(t.size(0) > 1 ? t.stride(0) : heads * groups * bytes_of);
+  return c;
+}
+
+// kv_store(cache, k, v, slots)
+TCRV_CALL(kv_store, 4) {
+  const at::Tensor &t = tensor(a[0]);
+  tcrv_cuda_kv_cache cache = kv_cache(t);
+  const char *text = "keys and values are (tokens, kv_heads, dim) with adjacent elements of a head";
+  const at::Tensor &k = head_rows(a[1], text), &v = head_rows(a[2], text);
+  const int type = activation_type(k);
+  if (v.scalar_type() != k.scalar_type())
+    fail(PyExc_TypeError, "keys and values differ in type");
+  if (k.sizes() != v.sizes() || k.size(1) != static_cast<int64_t>(cache.kv_heads) || k.size(2) != static_cast<int64_t>(cache.dim))
+    fail(PyExc_ValueError, "keys, values and the cache differ in shape");
+  const at::Tensor &slots = dense_beside(a[3], at::kLong, t);
+  same_device(t, k);
+  same_device(t, v);
+  if (slots.numel() != k.size(0))
+    fail(PyExc_ValueError, "one slot for each token");
+  const c10::cuda::CUDAGuard guard(t.device());
+  const cudaStream_t st = stream();
+  check(module, unlocked([&] {
+          cache.data = bytes(t);
+          return tcrv_cuda_kv_store_q4_0(type, static_cast<size_t>(k.size(0)), k.data_ptr(), static_cast<size_t>(k.stride(0)),
+                                         static_cast<size_t>(k.stride(1)), v.data_ptr(), static_cast<size_t>(v.stride(0)),
+                                         static_cast<size_t>(v.stride(1)), static_cast<const int64_t *>(slots.data_ptr()), &cache, st);
+        }),
+        "tcrv_cuda_kv_store_q4_0");
+  Py_INCREF(a[0]);
+  return a[0];
+}
+
+// kv_load(cache, slots, type code)
+TCRV_CALL(kv_load, 3) {
+  const at::Tensor &t = tensor(a[0]);
+  tcrv_cuda_kv_cache cache = kv_cache(t);
+  const at::Tensor &slots = dense_beside(a[1], at::kLong, t);
+  const int type = static_cast<int>(integer(a[2]));
+  const at::ScalarType scalar = type == TCRV_CUDA_TYPE_F32 ? at::kFloat : type == TCRV_CUDA_TYPE_F16 ? at::kHalf : at::kBFloat16;
+  const int64_t shape[3] = {slots.numel(), t.size(1), static_cast<int64_t>(cache.dim)};
+  at::Tensor k, v;
+  const c10::cuda::CUDAGuard guard(t.device());
+  const cudaStream_t st = stream();
+  check(module, unlocked([&] {
+          cache.data = bytes(t);
+          k = empty(shape, scalar, t);
+          v = empty(shape, scalar, t);
+          return tcrv_cuda_kv_load_q4_0(type, static_cast<size_t>(shape[0]), k.data_ptr(), v.data_ptr(),
+                                        static_cast<const int64_t *>(slots.data_ptr()), &cache, st);
+        }),
+        "tcrv_cuda_kv_load_q4_0");
+  return pair_of(std::move(k), std::move(v));
+}
+
+// attention(q, cache, block_table, kv_lens, first_rows or None, max_new, scale or None, window, out, with_lse, workspace)
+TCRV_CALL(attention, 11) {
+  const at::Tensor &q = head_rows(a[0], "queries are (rows, heads, dim) with adjacent elements of a head");
+  const at::Tensor &t = tensor(a[1]), &table = tensor(a[2]);
+  tcrv_cuda_attention_call c = {};
+  c.type = activation_type(q);
+  c.cache = kv_cache(t);
+  if (q.size(2) != static_cast<int64_t>(c.cache.dim))
+    fail(PyExc_ValueError, "queries and the cache differ in head size");
+  if (q.size(1) == 0 || q.size(1) % static_cast<int64_t>(c.cache.kv_heads) != 0)
+    fail(PyExc_ValueError, "the query heads must be a multiple of the cache's heads");
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1))
+    fail(PyExc_ValueError, "the block table is an int32 (requests, pages) matrix with adjacent pages");
+  const int64_t n = table.size(0), max_new = integer(a[5]), window = integer(a[7]);
+  const at::Tensor &lens = dense_beside(a[3], at::kInt, q);
+  same_device(q, t);
+  same_device(q, table);
+  if (lens.numel() != n)
+    fail(PyExc_ValueError, "one length for each request");
+  if (a[4] != Py_None) {
+    const at::Tensor &first = dense_beside(a[4], at::kInt, q);
+    if (first.numel() != n + 1)
+      fail(PyExc_ValueError, "first_rows has one entry for each request and one for the end");
+    c.first_rows = ints(first);
+  } else if (q.size(0) != n || max_new != 1) {
+    fail(PyExc_ValueError, "without first_rows each request has one row");
+  }
+  if (max_new < 1 || window < 0)
+    fail(PyExc_ValueError, "max_new must be positive and window not negative");
+  c.scale = a[6] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.cache.dim))) : static_cast<float>(real(a[6]));
+  const bool with_lse = truth(a[9]);
+  at::Tensor out, lse;
+  if (a[8] != Py_None)
+    same_device(q, out = head_output(a[8], q, q.size(0), q.size(1), q.size(2)));
+  Scratch ws(Py_None);
+  if (a[10] != Py_None) {
+    ws.tensor = dense(a[10], at::kByte);
+    same_device(q, ws.tensor);
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  const cudaStream_t st = stream();
+  check(module, unlocked([&] {
+          if (!out.defined())
+            out = empty(q.sizes(), q.scalar_type(), q);
+          if (with_lse)
+            lse = empty({q.size(0), q.size(1)}, at::kFloat, q);
+          c.requests = static_cast<size_t>(n);
+          c.rows = static_cast<size_t>(q.size(0));
+          c.heads = static_cast<size_t>(q.size(1));
+          c.max_new = static_cast<size_t>(max_new);
+          c.q = q.data_ptr();
+          c.q_row_stride = static_cast<size_t>(q.stride(0));
+          c.q_head_stride = static_cast<size_t>(q.stride(1));
+          c.out = out.data_ptr();
+          c.out_row_stride = static_cast<size_t>(out.stride(0));
+          c.out_head_stride = static_cast<size_t>(out.stride(1));
+          c.lse = with_lse ? floats(lse) : nullptr;
+          c.cache.data = bytes(t);
+          c.block_table = ints(table);
+          c.width = static_cast<size_t>(table.size(1));
+          c.table_stride = static_cast<size_t>(n > 1 ? table.stride(0) : table.size(1));
+          c.kv_lens = ints(lens);
+          c.window = static_cast<size_t>(window);
+          if (c.rows == 0 || c.requests == 0)
+            return static_cast<int>(TCRV_CUDA_OK);
+          ws.make(tcrv_cuda_attention_q4_0_workspace_bytes(&c), q);
+          c.workspace = ws.tensor.data_ptr();
+          c.workspace_bytes = ws.size();
+          return tcrv_cuda_attention_q4_0(&c, st);
+        }),
+        "tcrv_cuda_attention_q4_0");
+  return with_lse ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+}
+
 // bind(_check)
 TCRV_CALL(bind, 1) {
   Py_INCREF(a[0]);
@@ -519,7 +853,9 @@ PyMethodDef methods[] = {TCRV_METHOD(add),          TCRV_METHOD(dequantize),    
                          TCRV_METHOD(gemv),         TCRV_METHOD(gemv_group),       TCRV_METHOD(gemm),
                          TCRV_METHOD(gemm_prepared), TCRV_METHOD(sibling_dot_rows), TCRV_METHOD(rms_norm),
                          TCRV_METHOD(rope_apply),   TCRV_METHOD(vec_silu),         TCRV_METHOD(vec_scale_),
-                         TCRV_METHOD(repack_gemv),  TCRV_METHOD(bind),             {nullptr, nullptr, 0, nullptr}};
+                         TCRV_METHOD(repack_gemv),  TCRV_METHOD(rope),             TCRV_METHOD(kv_plan),
+                         TCRV_METHOD(kv_store),     TCRV_METHOD(kv_load),          TCRV_METHOD(attention),
+                         TCRV_METHOD(bind),         {nullptr, nullptr, 0, nullptr}};
 int traverse(PyObject *module, visitproc visit, void *arg) {
   Py_VISIT(state(module).check);
   return 0;
