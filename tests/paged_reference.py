@@ -113,7 +113,7 @@ def attention(q, cache, table, lens, first_rows, scale, window=0):
 HALF_STEP = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
 
 
-def attention_bounds(out, lse, weight, kind, largest_scale):
+def attention_bounds(out, lse, weight, kind, largest_scale, prompt=False):
     """How far a result may be from `attention`'s.  Scores: an f32 sum of products, in blocks of 32 and then over at most 8
     blocks (40 additions, each at most one step of 2^-23 where the tensor cores truncate), scaled (2^-23), the query in two fp16
     terms (2^-22).  A weight's relative error is twice the score's (its own, and the sum's) plus that of 2^x and the sum's
@@ -121,11 +121,16 @@ def attention_bounds(out, lse, weight, kind, largest_scale):
     absolute below fp16's normal range, times a quant of at most 8.  f32 calls round it to two terms, the second of which is off
     by at most 2^-25 too, after a power of two has lifted the largest scale D to 2^14 or more: 2^-25 / (2^14 / D) = 2^-39 D each.
     (A row whose heaviest tokens have quants of 8, that is values of 0, has nothing else to hide that behind.)  Last, the result's
-    own rounding."""
+    own rounding.
+    `prompt`: a call whose rows may go to the kernel that rounds every key and value, d * (n - 8), to fp16: half a step of 2^-11 on
+    each product and each term, and sums of up to 256 additions in one row of the product."""
     size, dot, count = weight
     score = dot * (41 * 2.0 ** -23 + 2.0 ** -22)
     relative = 2 * score + 2.0 ** -18
     absolute = count[..., None] * 8 * 2.0 ** -39 * largest_scale
+    if prompt:
+        score = dot * (256 * 2.0 ** -23 + 2.0 ** -22 + 2.0 ** -11)
+        relative = 2 * score + 2.0 ** -18 + 2.0 ** -11 + count * 2.0 ** -23
     if kind != "float32":
         relative = relative + 2.0 ** -11
         absolute = count[..., None] * 8 * 2.0 ** -25

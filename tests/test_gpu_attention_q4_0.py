@@ -15,8 +15,8 @@ def as_type(torch, x, kind):
     return t.cuda(), t.double().numpy()
 
 
-def check(got, lse, want, want_lse, weight, kind, spread=1.0):
-    bound, lse_bound = ref.attention_bounds(want, want_lse, weight, kind, 0.3 * spread)
+def check(got, lse, want, want_lse, weight, kind, spread=1.0, prompt=False):
+    bound, lse_bound = ref.attention_bounds(want, want_lse, weight, kind, 0.3 * spread, prompt)
     got = got.double().cpu().numpy()
     rows = ~np.isnan(want).any((1, 2))
     off = np.abs(got[rows] - want[rows])
@@ -30,7 +30,12 @@ def check(got, lse, want, want_lse, weight, kind, spread=1.0):
         assert (off <= lse_bound[rows][~empty]).all(), f"lse off by {off.max():.3g}"
 
 
-def run_case(torch, pkg, kind, lens, new, heads, kv_heads, dim, page_tokens, window=0, scale=None, seed=0, spread=1.0, q_std=1.0):
+def run_prompt(*a, **k):
+    run_case(*a, prompt=True, **k)
+
+
+def run_case(torch, pkg, kind, lens, new, heads, kv_heads, dim, page_tokens, window=0, scale=None, seed=0, spread=1.0, q_std=1.0, prompt=None):
+    prompt = prompt or kind != "float32" and dim in (64, 128) and max(new) * heads // kv_heads > 32
     rng = np.random.default_rng(seed)
     table, pages = ref.tables(rng, lens, page_tokens)
     cache = ref.random_cache(rng, pages, kv_heads, page_tokens, dim, spread)
@@ -42,7 +47,7 @@ def run_case(torch, pkg, kind, lens, new, heads, kv_heads, dim, page_tokens, win
                                   with_lse=True)
     pkg.check_device_errors()
     want, want_lse, weight = ref.attention(q64, cache, table, lens, first, dim ** -0.5 if scale is None else scale, window)
-    check(got, lse, want, want_lse, weight, kind, spread)
+    check(got, lse, want, want_lse, weight, kind, spread, prompt)
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -93,6 +98,103 @@ def test_many_short_requests(cuda, pkg, kind):
 def test_magnitudes_f32(cuda, pkg, spread, q_std, scale):
     # scales near both ends of fp16, queries far from 1, a peaked soft-max, a negative scale
     run_case(cuda, pkg, "float32", [300, 40], [1, 2], 4, 2, 128, 16, scale=scale, spread=spread, q_std=q_std, seed=8)
+
+
+# prompts: rows enough for the kernel whose operands are fp16 (16-bit calls, head sizes 64 and 128)
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 64), (4, 1, 128), (7, 1, 128), (6, 2, 64)])
+@pytest.mark.parametrize("lens,new", [([100], [100]), ([700, 5, 129, 40], [300, 1, 129, 2]), ([1500, 260], [33, 260])])
+def test_prompts(cuda, pkg, kind, heads, kv_heads, dim, lens, new):
+    run_prompt(cuda, pkg, kind, lens, new, heads, kv_heads, dim, 32, seed=heads + len(lens))
+
+
+@pytest.mark.parametrize("window", [1, 50, 128, 300])
+def test_prompts_with_windows(cuda, pkg, window):
+    run_prompt(cuda, pkg, "bfloat16", [700, 90], [400, 90], 4, 2, 128, 16, window=window, seed=window)
+
+
+def test_prompts_longer_than_their_context(cuda, pkg):
+    run_prompt(cuda, pkg, "float16", [20, 0, 300], [200, 140, 129], 2, 1, 128, 64, seed=1)
+
+
+@pytest.mark.parametrize("spread,q_std,scale", [(1e-3, 1.0, None), (2e5, 1e-6, None), (1.0, 3e4, 1e-5), (1.0, 20.0, None), (1.0, 1.0, -0.2)])
+def test_prompts_magnitudes(cuda, pkg, spread, q_std, scale):
+    run_prompt(cuda, pkg, "bfloat16", [300, 140], [100, 140], 4, 2, 64, 16, scale=scale, spread=spread, q_std=q_std, seed=8)
+
+
+def test_prompts_with_bad_values(cuda, pkg):
+    """Scales that are no numbers: behind the context they do not matter, in it they reach the rows that see their token only."""
+    rng = np.random.default_rng(4)
+    n, new = 300, 250
+    table, pages = ref.tables(rng, [n], 16)
+    table = np.concatenate((table, np.full((1, 3), -1, np.int32)), 1)
+    cache = ref.random_cache(rng, pages, 1, 16, 64)
+    q, _ = as_type(cuda, rng.standard_normal((new, 2, 64)), "bfloat16")
+    first, lens = cuda.tensor([0, new], dtype=cuda.int32, device="cuda"), cuda.tensor([n], dtype=cuda.int32, device="cuda")
+    t = cuda.from_numpy(table).cuda()
+    want = pkg.attention_q4_0(q, cuda.from_numpy(cache).cuda(), t, lens, first_rows=first, max_new=new)
+    _, _, _, kd, vd = ref.places(64)
+    for bits in (0x7c00, 0x7e00, 0xfc00):  # infinities, NaN
+        for at in (kd, vd):
+            for token in (300, 303, 280, 60):  # two behind the last token (in its page), two that some rows see
+                spoiled = cache.copy()
+                page = spoiled[table[0, token // 16], :, 0]
+                page[:, at[token % 16]], page[:, at[token % 16] + 1] = bits & 255, bits >> 8
+                got = pkg.attention_q4_0(q, cuda.from_numpy(spoiled).cuda(), t, lens, first_rows=first, max_new=new)
+                sees = max(0, min(new, token - (n - new)))  # rows before this one do not see the token
+                assert cuda.equal(got[:sees], want[:sees])
+                assert not bool(cuda.isfinite(got[sees:].float()).all(-1).any())
+
+
+def test_a_page_outside_the_cache_inside_a_prompt(cuda, pkg):
+    rng = np.random.default_rng(14)
+    table, pages = ref.tables(rng, [300], 16)
+    cache = ref.random_cache(rng, pages, 1, 16, 128)
+    table[0, 3], table[0, 15] = -3, pages + 5
+    q, q64 = as_type(cuda, rng.standard_normal((200, 2, 128)), "float16")
+    got, lse = pkg.attention_q4_0(q, cuda.from_numpy(cache).cuda(), cuda.from_numpy(table).cuda(), cuda.tensor([300], dtype=cuda.int32, device="cuda"),
+                                  first_rows=cuda.tensor([0, 200], dtype=cuda.int32, device="cuda"), max_new=200, with_lse=True)
+    want, want_lse, weight = ref.attention(q64, cache, table, [300], [0, 200], 128 ** -0.5)
+    check(got, lse, want, want_lse, weight, "float16", prompt=True)
+
+
+def test_prompts_strides_streams_and_graphs(cuda, pkg):
+    rng = np.random.default_rng(15)
+    lens64, new = [400, 300], [150, 300]
+    table, pages = ref.tables(rng, lens64, 16)
+    cache, t = cuda.from_numpy(ref.random_cache(rng, pages, 2, 16, 64)).cuda(), cuda.from_numpy(table).cuda()
+    q, _ = as_type(cuda, rng.standard_normal((sum(new), 4, 64)), "bfloat16")
+    first, lens = cuda.tensor([0, 150, 450], dtype=cuda.int32, device="cuda"), cuda.tensor(lens64, dtype=cuda.int32, device="cuda")
+    call = lambda x, **k: pkg.attention_q4_0(x, cache, t, lens, first_rows=first, max_new=300, **k)  # noqa: E731
+    want = call(q)
+    wide = cuda.zeros(450, 5, 67, dtype=q.dtype, device="cuda")
+    wide[:, 1:, 1:65] = q
+    out = cuda.full((4, 451, 70), 9.0, dtype=q.dtype, device="cuda")
+    call(wide[:, 1:, 1:65], out=out[:, :450, 3:67].transpose(0, 1))
+    assert cuda.equal(out[:, :450, 3:67].transpose(0, 1), want)
+    assert bool((out[..., :3] == 9).all()) and bool((out[..., 67:] == 9).all()) and bool((out[:, 450] == 9).all())
+    streams, results = [cuda.cuda.Stream() for _ in range(2)], []
+    cuda.cuda.synchronize()
+    for _ in range(5):
+        for s in streams:
+            with cuda.cuda.stream(s):
+                results.append(call(q))
+    cuda.cuda.synchronize()
+    assert all(cuda.equal(x, want) for x in results)
+    static = cuda.empty_like(q)
+    graph = cuda.cuda.CUDAGraph()
+    with cuda.cuda.graph(graph):
+        call(q, out=static)
+    graph.replay()
+    cuda.cuda.synchronize()
+    assert cuda.equal(static, want)
+    lens.copy_(cuda.tensor([200, 310], dtype=cuda.int32))
+    first.copy_(cuda.tensor([0, 2, 302], dtype=cuda.int32))  # one request falls to the other kernel
+    graph.replay()
+    cuda.cuda.synchronize()
+    assert cuda.equal(static[:302], call(q)[:302])
 
 
 def operands(torch, kind="bfloat16", lens=(50, 70, 20), heads=4, kv_heads=2, dim=64, page_tokens=16, seed=21):

@@ -1,5 +1,6 @@
 // Attention over the paged Q4_0 cache: choice of kernel, workspace, launches.
 #include "attention_columns.cuh"
+#include "attention_prefill.cuh"
 #include "launchers.h"
 
 namespace tcrv {
@@ -8,33 +9,54 @@ namespace {
 
 using namespace attention;
 
-// Columns (query rows times their f32 terms) that one pass over a context takes, in tiles of 8: the fewest that hold
-// all rows of a request, up to the tiles whose accumulators fit the registers.
-int column_tiles(const tcrv_cuda_attention_call &c) {
-  const int terms = c.type == TCRV_CUDA_TYPE_F32 ? 2 : 1;
-  const size_t columns = c.max_new * (c.heads / c.cache.kv_heads) * terms;
-  const int most = c.cache.dim <= 128 ? 4 : 2;
-  for (int t = 1; t < most; t *= 2)
-    if (columns <= static_cast<size_t>(8 * t))
-      return t;
-  return most;
-}
+// Rows of a request (new tokens * query heads of a kv head) from which its rows go to the prefill kernel, where there is one.
+constexpr size_t kPrefillRows = 33;
 
 struct Shape {
+  // the columns kernel
   int tiles, terms, rows;  // rows: query rows of a column group
   int grid;
+  long long most_rows;
+  // the prefill kernel
+  bool prefill;
+  int row_blocks, splits;
+  size_t parts;
+  size_t columns_bytes, prefill_offset, bytes;
 };
 
 Shape shape_of(const tcrv_cuda_attention_call &c) {
-  Shape s;
+  Shape s = {};
+  const size_t group = c.heads / c.cache.kv_heads, all = c.max_new * group;
   s.terms = c.type == TCRV_CUDA_TYPE_F32 ? 2 : 1;
-  s.tiles = column_tiles(c);
+  s.prefill = all >= kPrefillRows && c.type != TCRV_CUDA_TYPE_F32 && (c.cache.dim == 64 || c.cache.dim == 128);
+  const size_t rows = s.prefill ? kPrefillRows - 1 : all;
+  s.most_rows = static_cast<long long>(rows);
+  // columns (rows times their f32 terms) that one pass over a context takes, in tiles of 8: the fewest that hold all
+  // rows of a request, up to the tiles whose accumulators fit the registers
+  const int most_tiles = c.cache.dim <= 128 ? 4 : 2;
+  for (s.tiles = 1; s.tiles < most_tiles && rows * s.terms > static_cast<size_t>(8 * s.tiles);)
+    s.tiles *= 2;
   s.rows = s.tiles * 8 / s.terms;
   const size_t units = (c.width * c.cache.groups + kUnitGroups - 1) / kUnitGroups;
-  const size_t groups = (c.max_new * (c.heads / c.cache.kv_heads) + s.rows - 1) / s.rows;
+  const size_t groups = (rows + s.rows - 1) / s.rows;
   const double most = static_cast<double>(units ? units : 1) * groups * c.cache.kv_heads * c.requests / kWarps + 1;
   const int cap = sm_count() * ctas_per_sm(static_cast<int>(c.cache.dim / 32), s.tiles);
   s.grid = most < cap ? static_cast<int>(most) : cap;
+  s.columns_bytes = column_workspace_bytes(s.grid, s.rows, c.cache.dim);
+  s.prefill_offset = (s.columns_bytes + 255) / 256 * 256;
+  s.bytes = s.columns_bytes;
+  if (s.prefill) {
+    s.row_blocks = static_cast<int>((all + 2 * kTileRows - 1) / (2 * kTileRows));
+    const size_t items = static_cast<size_t>(s.row_blocks) * c.requests * c.cache.kv_heads;
+    // with fewer row blocks than half the SMs, each one's tokens are shared by several CTAs
+    const size_t tiles = (c.width * c.cache.groups + kTileGroups - 1) / kTileGroups;
+    size_t splits = items * 2 > static_cast<size_t>(sm_count()) ? 1 : sm_count() / items;
+    splits = splits > (tiles + 3) / 4 ? (tiles + 3) / 4 : splits;
+    s.splits = splits < 1 ? 1 : splits > 32 ? 32 : static_cast<int>(splits);
+    s.parts = items * s.splits;
+    if (s.splits > 1)
+      s.bytes = s.prefill_offset + prefill_workspace_bytes(s.parts, c.cache.dim);
+  }
   return s;
 }
 
@@ -71,21 +93,46 @@ int launch_dim(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
   return TCRV_CUDA_ERR_UNSUPPORTED;
 }
 
+template <int NB>
+int launch_prefill(const tcrv_cuda_attention_call &c, const Shape &s, const DeviceErrorWords &errors, cudaStream_t stream) {
+  if (s.parts > 0x7fffffff)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  PrefillParams p = {};
+  p.call = c;
+  p.call.workspace = static_cast<uint8_t *>(c.workspace) + s.prefill_offset;
+  p.group = static_cast<uint32_t>(c.heads / c.cache.kv_heads);
+  p.min_rows = static_cast<int32_t>(kPrefillRows);
+  p.row_blocks = s.row_blocks;
+  p.splits = s.splits;
+  p.errors = errors;
+  constexpr size_t smem = PrefillLayout<NB>::kBytes;
+  TCRV_CUDA_TRY(cudaFuncSetAttribute(prefill_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  TCRV_CUDA_TRY(launch_pdl(prefill_kernel<NB>, dim3(static_cast<unsigned>(s.parts)), kPrefillThreads, smem, stream, p));
+  if (s.splits > 1) {
+    const dim3 grid(2 * kTileRows / 8, static_cast<unsigned>(s.parts / s.splits));
+    TCRV_CUDA_TRY(launch_pdl(prefill_combine_kernel<NB>, grid, 256, 0, stream, p, static_cast<uint32_t>(s.parts)));
+  }
+  return TCRV_CUDA_OK;
+}
+
 }  // namespace
 
-size_t attention_workspace_bytes(const tcrv_cuda_attention_call &c) {
-  const Shape s = shape_of(c);
-  return column_workspace_bytes(s.grid, s.rows, c.cache.dim);
-}
+size_t attention_workspace_bytes(const tcrv_cuda_attention_call &c) { return shape_of(c).bytes; }
 
 int launch_attention_q4_0(const tcrv_cuda_attention_call &c, cudaStream_t stream) {
   const Shape s = shape_of(c);
   ColumnParams p = {};
   p.call = c;
   p.group = static_cast<uint32_t>(c.heads / c.cache.kv_heads);
+  p.most_rows = s.most_rows;
   const int st = device_error_words(&p.errors);
   if (st != TCRV_CUDA_OK)
     return st;
+  if (s.prefill) {
+    const int rc = c.cache.dim == 64 ? launch_prefill<2>(c, s, p.errors, stream) : launch_prefill<4>(c, s, p.errors, stream);
+    if (rc != TCRV_CUDA_OK)
+      return rc;
+  }
   switch (c.cache.dim) {
     case 64:
       return launch_dim<2>(p, s, stream);

@@ -31,7 +31,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct ColumnParams {
   tcrv_cuda_attention_call call;
-  uint32_t group;  // query heads to a kv head
+  uint32_t group;       // query heads to a kv head
+  long long most_rows;  // requests with more rows (new tokens * group) are another kernel's
   DeviceErrorWords errors;
 };
 
@@ -154,8 +155,7 @@ struct Request {
   int32_t rows, first_row, len, first_unit, units, column_groups;
 };
 
-__device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t r, int group_rows) {
-  const tcrv_cuda_attention_call &c = p.call;
+__device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &c, uint32_t group, uint32_t r, int group_rows) {
   Request q;
   long long first = c.first_rows ? c.first_rows[r] : r, end = c.first_rows ? c.first_rows[r + 1] : r + 1ll;
   if (first < 0)
@@ -176,7 +176,15 @@ __device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t 
   q.first_unit = static_cast<int32_t>(low / kUnitTokens);
   const int32_t units = static_cast<int32_t>((len + kUnitTokens - 1) / kUnitTokens) - q.first_unit;
   q.units = rows == 0 ? 0 : units < 1 ? 1 : units;  // (a request that sees nothing still writes its zeros)
-  q.column_groups = static_cast<int32_t>((rows * p.group + group_rows - 1) / group_rows);
+  q.column_groups = static_cast<int32_t>((rows * group + group_rows - 1) / group_rows);
+  return q;
+}
+
+// The same for the kernel of this file: requests with more rows than it is meant for have no units.
+__device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t r, int group_rows) {
+  Request q = load_request(p.call, p.group, r, group_rows);
+  if (static_cast<long long>(q.rows) * p.group > p.most_rows)
+    q.units = 0;
   return q;
 }
 

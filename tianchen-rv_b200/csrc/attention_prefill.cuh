@@ -1,0 +1,702 @@
+// Attention of many query rows per request (prompts) over the paged Q4_0 cache, fp16 and bf16 calls: tcgen05
+// products with their accumulators in tensor memory.
+//
+// A CTA takes 256 rows, two tiles of 128 (row = new token * heads of the kv head + head, so the heads that share a
+// cache head share its tiles), and walks over the context in tiles of 128 tokens:
+//   S = Q K^T (128 x 128, f32, TMEM)  ->  P = 2^(S * scale - m) (fp16, TMEM, over S)  ->  O += P V (128 x D, f32, TMEM).
+// Warps 0..3 and 4..7 are the soft-max of the two tiles, a thread to a row; warps 8..11 turn quants into the fp16
+// operands in shared memory, warp 12 issues the products.  While one tile's soft-max runs the other tile's products do.
+//
+// Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
+// scaled block by block without reading S and O once for every block of 32.  Query rows are fp16 after a power of two
+// (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A group with a scale so large that
+// its values leave fp16 is held at 1/16 and made good in S or in P.  The running maximum that P is relative to follows the
+// true one only when that has grown by more than 2^8: then O is rescaled, otherwise P just has values up to 2^8.
+#pragma once
+
+#include "attention_columns.cuh"
+#include "tcgen05.cuh"
+
+namespace tcrv {
+namespace attention {
+
+constexpr int kPrefillWarps = 13;
+constexpr int kPrefillThreads = 32 * kPrefillWarps;
+constexpr int kTileRows = 128;
+constexpr int kTileTokens = 128;
+constexpr int kTileGroups = kTileTokens / kGroupTokens;
+constexpr int kSlots = 4;  // tiles whose group flags are kept
+
+struct PrefillParams {
+  tcrv_cuda_attention_call call;
+  uint32_t group;
+  int32_t min_rows;      // requests with fewer rows (new tokens * group) are another kernel's
+  int32_t row_blocks;    // of a request at most
+  int32_t splits;        // CTAs that share the tokens of one row block
+  DeviceErrorWords errors;
+};
+
+// Workspace with splits > 1: (maximum, sum) and accumulators of each part's 256 rows.
+__host__ __device__ inline size_t prefill_sums_offset(size_t parts) { return parts * 2 * kTileRows * 2 * sizeof(float); }
+inline size_t prefill_workspace_bytes(size_t parts, size_t dim) {
+  return prefill_sums_offset(parts) + parts * 2 * kTileRows * dim * sizeof(float);
+}
+
+template <int NB>
+struct PrefillLayout {
+  static constexpr int kDim = 32 * NB;
+  static constexpr int kPanel = 128 * 128;                       // 128 rows of 128 bytes
+  static constexpr int kKeyBytes = kDim / 64 * kPanel;           // 128 tokens x D, K-major
+  static constexpr int kValueBytes = kTileTokens / 64 * kDim * 128;  // D x 128 tokens, K-major
+  static constexpr int kQuery = 0;
+  static constexpr int kKey = kQuery + 2 * kKeyBytes;
+  static constexpr int kValue = kKey + 2 * kKeyBytes;
+  static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
+  static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group]: tokens with a value scale that is no number
+  static constexpr int kBars = kPoison + kSlots * kTileGroups * 2;
+  static constexpr int kBarCount = 15;
+  static constexpr int kTmem = kBars + kBarCount * 8;
+  static constexpr int kAbort = kTmem + 4;
+  static constexpr int kBytes = kAbort + 4 + 1024;  // (the base is rounded up to 1024)
+};
+
+// barriers
+enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13 };
+
+// kind::f16, fp16 A and B (both K-major), f32 D.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
+// v[0..16) into 16 consecutive columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// One lane's share of a group as it lies in the cache.
+template <int NB>
+struct RawGroup {
+  uint32_t key[2][NB], value[2][NB];
+  uint32_t key_scale[2][NB / 2];  // tokens g, g + 8
+  uint32_t value_scale[2][NB];    // tokens (2t, 2t + 1), (2t + 8, 2t + 9)
+  bool there;
+};
+
+template <int N>
+__device__ __forceinline__ void load_global(uint32_t (&w)[N], const uint8_t *p) {
+  if constexpr (N == 1)
+    w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+  else if constexpr (N == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    static_assert(N == 4, "words to a load");
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
+  using L = PrefillLayout<NB>;
+  constexpr int kDim = L::kDim;
+  extern __shared__ uint8_t prefill_smem[];
+  uint8_t *smem = prefill_smem + ((1024u - (smem_addr(prefill_smem) & 1023u)) & 1023u);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
+  uint32_t *tmem_word = reinterpret_cast<uint32_t *>(smem + L::kTmem);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + L::kAbort);
+  volatile uint8_t *flags = smem + L::kFlags;
+  volatile uint16_t *poison = reinterpret_cast<volatile uint16_t *>(smem + L::kPoison);
+  const tcrv_cuda_attention_call &c = p.call;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_enter();
+  // ---- what this CTA does: the longest row blocks come first
+  const uint32_t kv_heads = static_cast<uint32_t>(c.cache.kv_heads);
+  uint32_t id = blockIdx.x;
+  const int part = static_cast<int>(id % p.splits);
+  id /= p.splits;
+  const uint32_t r = id % static_cast<uint32_t>(c.requests);
+  id /= static_cast<uint32_t>(c.requests);
+  const uint32_t head = id % kv_heads;
+  const int32_t from_end = static_cast<int32_t>(id / kv_heads);
+  const Request q = load_request(p.call, p.group, r, 1 << 30);
+  const int32_t rows = q.rows * static_cast<int32_t>(p.group);
+  const int32_t blocks = (rows + 2 * kTileRows - 1) / (2 * kTileRows);
+  if (rows < p.min_rows || from_end >= blocks)
+    return;
+  const int32_t block = blocks - 1 - from_end, pair0 = block * 2 * kTileRows;
+  const int tiles_q = rows - pair0 > kTileRows ? 2 : 1;
+  const int32_t last_pair = min(rows, pair0 + 2 * kTileRows) - 1;
+  const int32_t before = q.len - q.rows;  // position of the request's first row
+  const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
+  const int32_t see_to = before + last_pair / static_cast<int32_t>(p.group);  // the last row sees furthest
+  const int32_t see_from = window ? max(0, before + pair0 / static_cast<int32_t>(p.group) - window + 1) : 0;
+  int32_t tile_begin = see_from / kTileTokens, tile_end = see_to < 0 ? tile_begin : see_to / kTileTokens + 1;
+  if (p.splits > 1) {
+    const int32_t n = tile_end - tile_begin, b = tile_begin;
+    tile_begin = b + static_cast<int32_t>(static_cast<int64_t>(n) * part / p.splits);
+    tile_end = b + static_cast<int32_t>(static_cast<int64_t>(n) * (part + 1) / p.splits);
+  }
+  const int tiles = tile_end - tile_begin;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars[kBarQuery], 4 * tiles_q);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[kBarKeyFull + i], 4);
+      mbar_init(&bars[kBarKeyFree + i], 1);
+      mbar_init(&bars[kBarValueFull + i], 4);
+      mbar_init(&bars[kBarValueFree + i], 1);
+      mbar_init(&bars[kBarScores + i], 1);
+      mbar_init(&bars[kBarWeights + i], 4);
+      mbar_init(&bars[kBarSums + i], 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_word, 512);
+    tmem_relinquish_alloc_permit();
+  }
+  tcgen05_fence_before_thread_sync();
+  __syncthreads();
+  tcgen05_fence_after_thread_sync();
+  const uint32_t tmem = *tmem_word;
+  // scores of tile i at columns 128 i (its weights over their first half), sums at 256 + D i
+  const auto wait = [&](int bar, uint32_t parity) {
+    if (mbar_wait_bounded(&bars[bar], parity & 1u, abort_flag))
+      return true;
+    if (*abort_flag == 0) {
+      *abort_flag = 1;
+      if (lane == 0)
+        raise_device_error(p.errors, kDevErrBarrierTimeout);
+    }
+    return false;
+  };
+
+  if (warp < 8) {
+    // ================================================================ soft-max of one tile
+    const int tile = warp >> 2;
+    if (tile < tiles_q) {
+      // ---- the query operand: this warp's 32 rows, in the key operand's order of elements, and a power of two that lifts
+      // the largest element into [2^14, 2^15)
+      const int row0 = (warp & 3) * 32;
+      const uint32_t quadrant = static_cast<uint32_t>(row0) << 16;
+      int my_lift = 0;
+      {
+        uint8_t *operand = smem + L::kQuery + tile * L::kKeyBytes;
+        const int e = lane & 15, t = e >> 2, f = ((lane >> 4) << 2) | ((e & 1) << 1) | ((e >> 1) & 1);
+        constexpr int kBatch = 8;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32; i0 += kBatch) {
+          float x[kBatch][NB];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int32_t pair = pair0 + tile * kTileRows + row0 + i0 + i, token = pair / static_cast<int32_t>(p.group);
+            const size_t at = static_cast<size_t>(q.first_row + token) * c.q_row_stride +
+                              (static_cast<size_t>(head) * p.group + (pair - token * p.group)) * c.q_head_stride;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              x[i][b] = pair < rows ? load_typed(c.q, at + b * 32 + lane, c.type) : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            float top = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              top = fmaxf(top, fabsf(x[i][b]));
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            int k = 0;
+            if (top > 0.0f && top < INFINITY)
+              k = min(120, 14 - ilogbf(top));
+            const float lift = exp2f(static_cast<float>(k)) * (c.scale < 0.0f ? -1.0f : 1.0f);
+            const int row = row0 + i0 + i;
+            if (lane == i0 + i)
+              my_lift = k;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const int chunk = 2 * t + (b & 1);
+              *reinterpret_cast<__half *>(operand + (b >> 1) * L::kPanel + row * 128 + ((chunk ^ (row & 7)) << 4) + f * 2) =
+                  __float2half_rn(x[i][b] * lift);
+            }
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars[kBarQuery]);
+      }
+      const int32_t pair = pair0 + tile * kTileRows + row0 + lane, token = pair / static_cast<int32_t>(p.group);
+      const int32_t position = pair < rows ? before + token : -1;
+      const float scale = fabsf(c.scale) * kLog2e * exp2f(static_cast<float>(-my_lift));
+      const uint32_t scores = tmem + quadrant + tile * 128, sums = tmem + quadrant + 256 + tile * kDim;
+      const int32_t tile_pair0 = pair0 + tile * kTileRows;
+      const int32_t tile_from = window ? before + (min(rows, tile_pair0 + kTileRows) - 1) / static_cast<int32_t>(p.group) - window + 1 : 0;
+      const int32_t tile_to = before + tile_pair0 / static_cast<int32_t>(p.group);
+      float m = -INFINITY, l = 0.0f;
+      bool going = true;
+#pragma unroll 1
+      for (int j = 0; j < tiles && going; ++j) {
+        if (!wait(kBarScores + tile, j))
+          break;
+        tcgen05_fence_after_thread_sync();
+        const int32_t token0 = (tile_begin + j) * kTileTokens;
+        const int slot = j % kSlots;
+        const uint64_t group_flags = *reinterpret_cast<volatile uint64_t *>(smem + L::kFlags + slot * kTileGroups);
+        const bool whole = group_flags == 0x0101010101010101ull && token0 >= tile_from && token0 + kTileTokens - 1 <= tile_to;
+        // what a score counts as, with the mask and the groups' flags
+        const auto masked = [&](float s, int column) {
+          const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (column / kGroupTokens))) & 0xffu;
+          const int32_t at = token0 + column;
+          s *= scale * ((flag & 2u) ? 16.0f : 1.0f);
+          return (flag & 1u) && at <= position && !(window && at <= position - window) ? s : -INFINITY;
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t s[32];
+          tmem_ld_32x32b<32>(scores + ch * 32, s);
+          tmem_ld_wait();
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              top = fmaxf(top, __uint_as_float(s[i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              top = fmaxf(top, masked(__uint_as_float(s[i]), ch * 32 + i));
+          }
+        }
+        if (whole)
+          top *= scale;
+        const bool grown = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, grown)) {
+          const float now = grown ? top : m, alpha = grown ? exp2_fast(m - now) : 1.0f;
+          m = now;
+          l *= alpha;
+          if (j > 0) {
+            if (!wait(kBarSums + tile, j - 1))
+              break;
+            tcgen05_fence_after_thread_sync();
+#pragma unroll
+            for (int ch = 0; ch < kDim / 16; ++ch) {
+              uint32_t o[16];
+              tmem_ld_32x32b<16>(sums + ch * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32b_x16(sums + ch * 16, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t s[32], w[16];
+          tmem_ld_32x32b<32>(scores + ch * 32, s);
+          tmem_ld_wait();
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float a = exp2_fast(fmaf(__uint_as_float(s[i]), scale, -base));
+              const float b = exp2_fast(fmaf(__uint_as_float(s[i + 1]), scale, -base));
+              l += a + b;
+              w[i / 2] = half2_bits(__floats2half2_rn(a, b));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float a = exp2_fast(masked(__uint_as_float(s[i]), ch * 32 + i) - base);
+              float b = exp2_fast(masked(__uint_as_float(s[i + 1]), ch * 32 + i + 1) - base);
+              l += a + b;
+              const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * ((ch * 32 + i) / kGroupTokens))) & 0xffu;
+              if (flag & 4u) {
+                a *= 16.0f;
+                b *= 16.0f;
+              }
+              w[i / 2] = half2_bits(__floats2half2_rn(a, b));
+            }
+          }
+          tmem_st_32x32b_x16(scores + ch * 16, w);
+        }
+        if (group_flags & 0x0808080808080808ull) {  // a value that is no number: the rows that see its token are none either
+          for (int i = 0; i < kTileTokens; ++i) {
+            const int32_t at = token0 + i;
+            if (((poison[slot * kTileGroups + i / kGroupTokens] >> (i % kGroupTokens)) & 1) && at <= position && !(window && at <= position - window))
+              l = NAN;
+          }
+        }
+        tmem_st_wait();
+        tcgen05_fence_before_thread_sync();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars[kBarWeights + tile]);
+      }
+      // ---- the row's result; element n of the sums is d = 32 (n / 32) + 16 ((n >> 4) & 1) + 2 (n & 7) + ((n >> 3) & 1)
+      bool done = tiles > 0 && *abort_flag == 0;
+      if (done) {
+        done = wait(kBarSums + tile, tiles - 1);
+        tcgen05_fence_after_thread_sync();
+      }
+      const bool mine = pair < rows;
+      const size_t q_head = static_cast<size_t>(head) * p.group + (pair - token * static_cast<int32_t>(p.group));
+      const size_t at = static_cast<size_t>(q.first_row + token) * c.out_row_stride + q_head * c.out_head_stride;
+      const bool vector = (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0 && ((c.out_row_stride | c.out_head_stride) & 7u) == 0;
+      const size_t slot = (static_cast<size_t>(blockIdx.x) * 2 + tile) * kTileRows + row0 + lane;
+      float *part_sums = p.splits > 1 ? reinterpret_cast<float *>(static_cast<uint8_t *>(c.workspace) + prefill_sums_offset(gridDim.x)) + slot * kDim : nullptr;
+      const float factor = p.splits > 1 ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          o[i] = 0;
+        if (done) {
+          tmem_ld_32x32b<32>(sums + b * 32, o);
+          tmem_ld_wait();
+        }
+        float y[32];
+#pragma unroll
+        for (int d = 0; d < 32; ++d) {
+          const float v = __uint_as_float(o[(d >> 4) * 16 + (d & 1) * 8 + ((d & 15) >> 1)]);
+          y[d] = l > 0.0f || l != l ? v * factor : 0.0f;
+        }
+        if (mine) {
+          if (part_sums != nullptr) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4)
+              *reinterpret_cast<float4 *>(part_sums + b * 32 + d) = make_float4(y[d], y[d + 1], y[d + 2], y[d + 3]);
+          } else if (vector) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (c.type == TCRV_CUDA_TYPE_F16) {
+                  w[i] = half2_bits(__floats2half2_rn(y[d + 2 * i], y[d + 2 * i + 1]));
+                } else {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(y[d + 2 * i], y[d + 2 * i + 1]);
+                  memcpy(&w[i], &h, 4);
+                }
+              }
+              *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(c.out) + at + b * 32 + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int d = 0; d < 32; ++d)
+              store_typed(c.out, at + b * 32 + d, c.type, y[d]);
+          }
+        }
+      }
+      if (mine) {
+        if (part_sums != nullptr)
+          *reinterpret_cast<float2 *>(static_cast<float *>(c.workspace) + slot * 2) = make_float2(m, l);
+        else if (c.lse != nullptr)
+          c.lse[static_cast<size_t>(q.first_row + token) * c.heads + q_head] =
+              l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      }
+    }
+  } else if (warp < 12) {
+    // ================================================================ quants -> fp16 operands
+    const int w = warp - 8, g = lane >> 2, t = lane & 3;
+    const uint32_t per_page = static_cast<uint32_t>(c.cache.groups);
+    const int32_t groups = (q.len + kGroupTokens - 1) / kGroupTokens;
+    const int32_t *table = c.block_table + r * c.table_stride;
+    // group i (0 or 1) of this warp in tile j
+    const auto group_of = [&](int j, int i) { return (tile_begin + j) * kTileGroups + w + 4 * i; };
+    const auto page_of = [&](int j, int i) -> int32_t {
+      const int32_t at = group_of(j, i);
+      return j < tiles && at < groups ? table[static_cast<uint32_t>(at) / per_page] : -1;
+    };
+    const auto fetch = [&](RawGroup<NB> &raw, int j, int i, int32_t page) {
+      raw.there = page >= 0 && static_cast<size_t>(page) < c.cache.pages;
+      if (raw.there) {
+        const uint32_t in_page = static_cast<uint32_t>(group_of(j, i)) % per_page;
+        const uint8_t *at = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
+                            (static_cast<size_t>(head) * per_page + in_page) * (18 * kDim);
+        load_global<NB>(raw.key[0], at + lane * NB * 4);
+        load_global<NB>(raw.key[1], at + 128 * NB + lane * NB * 4);
+        load_global<NB>(raw.value[0], at + 256 * NB + lane * NB * 4);
+        load_global<NB>(raw.value[1], at + 384 * NB + lane * NB * 4);
+        load_global<NB / 2>(raw.key_scale[0], at + 512 * NB + g * NB * 2);
+        load_global<NB / 2>(raw.key_scale[1], at + 512 * NB + (g + 8) * NB * 2);
+        load_global<NB>(raw.value_scale[0], at + 544 * NB + 2 * t * NB * 2);
+        load_global<NB>(raw.value_scale[1], at + 544 * NB + (2 * t + 8) * NB * 2);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            raw.key[h][b] = raw.value[h][b] = raw.value_scale[h][b] = 0;
+#pragma unroll
+          for (int b = 0; b < NB / 2; ++b)
+            raw.key_scale[h][b] = 0;
+        }
+      }
+    };
+    const auto half_of = [](const uint32_t *words, int i) -> uint32_t { return (words[i >> 1] >> (16 * (i & 1))) & 0xffffu; };
+    RawGroup<NB> now[2], ahead[2];
+    int32_t pages[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      fetch(ahead[i], 0, i, page_of(0, i));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      pages[i] = page_of(1, i);
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j & 1, slot = j % kSlots;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        now[i] = ahead[i];
+        fetch(ahead[i], j + 1, i, pages[i]);
+        pages[i] = page_of(j + 2, i);
+      }
+      if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
+        break;
+      // ---- scales: none for tokens behind the context, the others checked
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int32_t first = group_of(j, i) * kGroupTokens, left = q.len - first;
+        uint32_t big_key = 0, big_value = 0, bad = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (g + 8 * h >= left) {
+#pragma unroll
+            for (int b = 0; b < NB / 2; ++b)
+              now[i].key_scale[h][b] = 0;
+          }
+          uint32_t keep = (2 * t + 8 * h < left ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < left ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int b = 0; b < NB / 2; ++b)
+            big_key |= ((now[i].key_scale[h][b] & 0x7fff7fffu) + 0x10001000u) & 0x80008000u;  // |d| >= 2^13: 8 d leaves fp16
+          // pairs of tokens side by side
+          uint32_t pair[NB];
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            pair[b] = (half_of(now[i].value_scale[h], b) | (half_of(now[i].value_scale[h], NB + b) << 16)) & keep;
+            const uint32_t size = pair[b] & 0x7fff7fffu;
+            if ((size & 0x7c00u) == 0x7c00u) {
+              bad |= 1u << (2 * t + 8 * h);
+              pair[b] &= 0xffff0000u;
+            }
+            if ((size & 0x7c000000u) == 0x7c000000u) {
+              bad |= 2u << (2 * t + 8 * h);
+              pair[b] &= 0xffffu;
+            }
+            big_value |= ((pair[b] & 0x7fff7fffu) + 0x10001000u) & 0x80008000u;
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            now[i].value_scale[h][b] = pair[b];
+        }
+        const bool some_key = __any_sync(0xffffffffu, big_key != 0), some_value = __any_sync(0xffffffffu, big_value != 0);
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          flags[slot * kTileGroups + w + 4 * i] =
+              static_cast<uint8_t>((now[i].there ? 1 : 0) | (some_key ? 2 : 0) | (some_value ? 4 : 0) | (bad ? 8 : 0));
+          poison[slot * kTileGroups + w + 4 * i] = static_cast<uint16_t>(bad);
+        }
+        if (some_key || some_value) {
+          const __half2 sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < NB / 2; ++b)
+              if (some_key)
+                now[i].key_scale[h][b] = half2_bits(__hmul2(bits_half2(now[i].key_scale[h][b]), sixteenth));
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              if (some_value)
+                now[i].value_scale[h][b] = half2_bits(__hmul2(bits_half2(now[i].value_scale[h][b]), sixteenth));
+          }
+        }
+      }
+      // ---- keys: a word's 8 elements are 16 bytes of the token's row; neighbouring lanes' chunks fall on different banks
+      uint8_t *keys = smem + L::kKey + stage * L::kKeyBytes;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = (w + 4 * i) * kGroupTokens + h * 8 + g;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint32_t word = now[i].key[h][b], d = half_of(now[i].key_scale[h], b);
+            const __half2 scale = bits_half2(d | (d << 16));
+            const uint4 v = make_uint4(half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
+                                       half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
+                                       half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
+                                       half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale)));
+            *reinterpret_cast<uint4 *>(keys + (b >> 1) * L::kPanel + row * 128 + (((2 * t + (b & 1)) ^ (row & 7)) << 4)) = v;
+          }
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars[kBarKeyFull + stage]);
+      // ---- values, transposed: row n of the operand is an element, its columns the tokens
+      if (j >= 2 && !wait(kBarValueFree + stage, (j >> 1) - 1))
+        break;
+      uint8_t *values = smem + L::kValue + stage * L::kValueBytes;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int group = w + 4 * i;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int chunk = (group & 3) * 2 + h;
+          uint8_t *panel = values + (group >> 2) * (kDim * 128) + ((chunk ^ g) << 4) + t * 4;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint32_t word = now[i].value[h][b];
+            const __half2 scale = bits_half2(now[i].value_scale[h][b]);
+            const uint32_t v[4] = {half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
+                                   half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
+                                   half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
+                                   half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale))};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint32_t *>(panel + ((b * 4 + k) * 8 + g) * 128) = v[k];
+          }
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars[kBarValueFull + stage]);
+    }
+  } else if (tiles > 0) {
+    // ================================================================ products: one lane issues
+    const uint32_t base = smem_addr(smem);
+    constexpr uint32_t kScoreDesc = umma_idesc_f16(kTileRows, kTileTokens), kSumDesc = umma_idesc_f16(kTileRows, kDim);
+    const bool leader = elect_one();
+    const auto score = [&](int tile, int stage) {
+      const uint64_t a = umma_desc_k_major_sw128(base + L::kQuery + tile * L::kKeyBytes);
+      const uint64_t b = umma_desc_k_major_sw128(base + L::kKey + stage * L::kKeyBytes);
+#pragma unroll
+      for (int k = 0; k < kDim / 16; ++k) {
+        const uint32_t at = (k / 4) * (L::kPanel >> 4) + (k % 4) * 2;
+        umma_f16_ss(tmem + tile * 128, a + at, b + at, kScoreDesc, k > 0);
+      }
+      umma_commit(&bars[kBarScores + tile]);
+    };
+    const auto sum = [&](int tile, int stage, bool add) {
+      const uint64_t b = umma_desc_k_major_sw128(base + L::kValue + stage * L::kValueBytes);
+#pragma unroll
+      for (int k = 0; k < kTileTokens / 16; ++k) {
+        const uint32_t at = (k / 4) * ((kDim * 128) >> 4) + (k % 4) * 2;
+        umma_f16_ts(tmem + 256 + tile * kDim, tmem + tile * 128 + k * 8, b + at, kSumDesc, add || k > 0);
+      }
+      umma_commit(&bars[kBarSums + tile]);
+    };
+    bool good = wait(kBarQuery, 0) && wait(kBarKeyFull, 0);
+    tcgen05_fence_after_thread_sync();
+    if (good && leader) {
+      for (int i = 0; i < tiles_q; ++i)
+        score(i, 0);
+      umma_commit(&bars[kBarKeyFree]);
+    }
+#pragma unroll 1
+    for (int j = 0; j < tiles && good; ++j) {
+      const int stage = j & 1, next = (j + 1) & 1;
+      good = wait(kBarValueFull + stage, j >> 1);
+      for (int i = 0; i < tiles_q && good; ++i) {
+        good = wait(kBarWeights + i, j);
+        if (i == 0 && good && j + 1 < tiles)
+          good = wait(kBarKeyFull + next, (j + 1) >> 1);
+        tcgen05_fence_after_thread_sync();
+        if (good && leader) {
+          sum(i, stage, j > 0);
+          if (i == tiles_q - 1)
+            umma_commit(&bars[kBarValueFree + stage]);
+          if (j + 1 < tiles) {
+            score(i, next);
+            if (i == tiles_q - 1)
+              umma_commit(&bars[kBarKeyFree + next]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  // ---- the tensor memory goes back when every role is through with it
+  tcgen05_fence_before_thread_sync();
+  __syncthreads();
+  tcgen05_fence_after_thread_sync();
+  if (warp == 12)
+    tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of a row block: one warp per row.
+template <int NB>
+__global__ void __launch_bounds__(256) prefill_combine_kernel(const __grid_constant__ PrefillParams p, uint32_t parts) {
+  constexpr int kDim = 32 * NB;
+  pdl_enter();
+  const tcrv_cuda_attention_call &c = p.call;
+  const uint32_t kv_heads = static_cast<uint32_t>(c.cache.kv_heads);
+  const int lane = threadIdx.x & 31;
+  uint32_t id = blockIdx.y;
+  const uint32_t first_part = id * p.splits;
+  const uint32_t r = id % static_cast<uint32_t>(c.requests);
+  id /= static_cast<uint32_t>(c.requests);
+  const uint32_t head = id % kv_heads;
+  const int32_t from_end = static_cast<int32_t>(id / kv_heads);
+  const Request q = load_request(p.call, p.group, r, 1 << 30);
+  const int32_t rows = q.rows * static_cast<int32_t>(p.group), blocks = (rows + 2 * kTileRows - 1) / (2 * kTileRows);
+  if (rows < p.min_rows || from_end >= blocks)
+    return;
+  const int32_t pair0 = (blocks - 1 - from_end) * 2 * kTileRows, row = static_cast<int32_t>(blockIdx.x * 8 + (threadIdx.x >> 5)), pair = pair0 + row;
+  if (pair >= rows)
+    return;
+  const float2 *stats = static_cast<const float2 *>(c.workspace);
+  const float *sums = reinterpret_cast<const float *>(static_cast<const uint8_t *>(c.workspace) + prefill_sums_offset(parts));
+  const auto slot = [&](int i) { return (static_cast<size_t>(first_part + i) * 2 * kTileRows) + row; };
+  float top = -INFINITY;
+  for (int i = 0; i < p.splits; ++i)
+    top = fmaxf(top, stats[slot(i)].x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, sum[NB] = {};
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 ml = stats[slot(i)];
+    const float f = exp2_fast(ml.x - base);
+    total = fmaf(f, ml.y, total);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      sum[b] = fmaf(f, sums[slot(i) * kDim + b * 32 + lane], sum[b]);
+  }
+  const int32_t token = pair / static_cast<int32_t>(p.group);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    write_row(c, q.first_row + token, head * p.group + (pair - token * p.group), b * 32 + lane, sum[b], total, top);
+}
+
+}  // namespace attention
+}  // namespace tcrv
