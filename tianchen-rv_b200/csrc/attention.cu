@@ -1,4 +1,6 @@
 // Attention over the paged Q4_0 cache: choice of kernel, workspace, launches.
+#include <atomic>
+
 #include "attention_columns.cuh"
 #include "attention_prefill.cuh"
 #include "launchers.h"
@@ -60,11 +62,35 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   return s;
 }
 
+// What a kernel needs once on each device: its shared memory, and for one that splits its registers the proof that a block
+// starts with as many (a block with fewer would wait for them for ever).
+struct Configured {
+  std::atomic<bool> done[64];
+};
+int configure(Configured &state, const void *kernel, size_t smem, int threads, int registers) {
+  int dev = 0;
+  TCRV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (!state.done[dev]) {
+    cudaFuncAttributes attributes;
+    TCRV_CUDA_TRY(cudaFuncGetAttributes(&attributes, kernel));
+    if (attributes.numRegs * threads < registers)
+      return TCRV_CUDA_ERR_UNSUPPORTED;
+    TCRV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    state.done[dev] = true;
+  }
+  return TCRV_CUDA_OK;
+}
+
 template <int NB, int NT, int TERMS>
 int launch_columns(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
   constexpr size_t smem = ColumnLayout<NB, NT, TERMS>::kBytes;
   auto *kernel = columns_kernel<NB, NT, TERMS>;
-  TCRV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  static Configured state;
+  const int st = configure(state, reinterpret_cast<const void *>(kernel), smem, kThreads, 0);
+  if (st != TCRV_CUDA_OK)
+    return st;
   TCRV_CUDA_TRY(launch_pdl(kernel, s.grid, kThreads, smem, stream, p));
   if (s.grid > 1) {
     const dim3 grid(static_cast<unsigned>(s.grid), static_cast<unsigned>(s.rows < 8 ? s.rows : 8));
@@ -106,7 +132,11 @@ int launch_prefill(const tcrv_cuda_attention_call &c, const Shape &s, const Devi
   p.splits = s.splits;
   p.errors = errors;
   constexpr size_t smem = PrefillLayout<NB>::kBytes;
-  TCRV_CUDA_TRY(cudaFuncSetAttribute(prefill_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  static Configured state;
+  const int st = configure(state, reinterpret_cast<const void *>(prefill_kernel<NB>), smem, kPrefillThreads,
+                           128 * (2 * kSoftmaxRegs + 2 * kQuantRegs + kProductRegs));
+  if (st != TCRV_CUDA_OK)
+    return st;
   TCRV_CUDA_TRY(launch_pdl(prefill_kernel<NB>, dim3(static_cast<unsigned>(s.parts)), kPrefillThreads, smem, stream, p));
   if (s.splits > 1) {
     const dim3 grid(2 * kTileRows / 8, static_cast<unsigned>(s.parts / s.splits));

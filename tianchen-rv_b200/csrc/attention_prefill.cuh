@@ -4,8 +4,8 @@
 // A CTA takes 256 rows, two tiles of 128 (row = new token * heads of the kv head + head, so the heads that share a
 // cache head share its tiles), and walks over the context in tiles of 128 tokens:
 //   S = Q K^T (128 x 128, f32, TMEM)  ->  P = 2^(S * scale - m) (fp16, TMEM, over S)  ->  O += P V (128 x D, f32, TMEM).
-// Warps 0..3 and 4..7 are the soft-max of the two tiles, a thread to a row; warps 8..11 turn quants into the fp16
-// operands in shared memory, warp 12 issues the products.  While one tile's soft-max runs the other tile's products do.
+// Warps 0..3 and 4..7 are the soft-max of the two tiles, a thread to a row; warps 8..15 turn quants into the fp16
+// operands in shared memory, warp 16 issues the products.  While one tile's soft-max runs the other tile's products do.
 //
 // Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
 // scaled block by block without reading S and O once for every block of 32.  Query rows are fp16 after a power of two
@@ -20,8 +20,12 @@
 namespace tcrv {
 namespace attention {
 
-constexpr int kPrefillWarps = 13;
-constexpr int kPrefillThreads = 32 * kPrefillWarps;
+constexpr int kQuantWarps = 8;
+constexpr int kProductWarp = 16;  // (the first of a warpgroup of which it alone has work)
+constexpr int kPrefillThreads = 640;
+// Registers: the block starts with 96 a thread; the soft-max takes over what the products' warpgroup can do without.
+constexpr int kStartRegs = 96, kSoftmaxRegs = 136, kQuantRegs = 88, kProductRegs = 32;
+static_assert(2 * kSoftmaxRegs + 2 * kQuantRegs + kProductRegs <= 5 * kStartRegs, "registers the block does not have");
 constexpr int kTileRows = 128;
 constexpr int kTileTokens = 128;
 constexpr int kTileGroups = kTileTokens / kGroupTokens;
@@ -98,6 +102,40 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t"
+      "}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t"
+      "}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // One lane's share of a group as it lies in the cache.
 template <int NB>
 struct RawGroup {
@@ -168,9 +206,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   if (threadIdx.x == 0) {
     mbar_init(&bars[kBarQuery], 4 * tiles_q);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars[kBarKeyFull + i], 4);
+      mbar_init(&bars[kBarKeyFull + i], kQuantWarps);
       mbar_init(&bars[kBarKeyFree + i], 1);
-      mbar_init(&bars[kBarValueFull + i], 4);
+      mbar_init(&bars[kBarValueFull + i], kQuantWarps);
       mbar_init(&bars[kBarValueFree + i], 1);
       mbar_init(&bars[kBarScores + i], 1);
       mbar_init(&bars[kBarWeights + i], 4);
@@ -179,7 +217,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 12) {
+  if (warp == kProductWarp) {
     tmem_alloc(tmem_word, 512);
     tmem_relinquish_alloc_permit();
   }
@@ -200,51 +238,76 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   };
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ================================================================ soft-max of one tile
     const int tile = warp >> 2;
     if (tile < tiles_q) {
       // ---- the query operand: this warp's 32 rows, in the key operand's order of elements, and a power of two that lifts
-      // the largest element into [2^14, 2^15)
+      // the largest element into [2^14, 2^15).  kDim / 8 lanes to a row, eight elements to a lane.
       const int row0 = (warp & 3) * 32;
       const uint32_t quadrant = static_cast<uint32_t>(row0) << 16;
       int my_lift = 0;
       {
+        constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = 8;
         uint8_t *operand = smem + L::kQuery + tile * L::kKeyBytes;
-        const int e = lane & 15, t = e >> 2, f = ((lane >> 4) << 2) | ((e & 1) << 1) | ((e >> 1) & 1);
-        constexpr int kBatch = 8;
+        const int sub = lane % kLanes, b = sub >> 2, high = (sub >> 1) & 1, t = (sub & 1) * 2;
+        const bool vector = (reinterpret_cast<uintptr_t>(c.q) & 15u) == 0 && ((c.q_row_stride | c.q_head_stride) & 7u) == 0;
+        const float sign = c.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll 1
-        for (int i0 = 0; i0 < 32; i0 += kBatch) {
-          float x[kBatch][NB];
+        for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+          uint4 raw[kBatch];
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
-            const int32_t pair = pair0 + tile * kTileRows + row0 + i0 + i, token = pair / static_cast<int32_t>(p.group);
-            const size_t at = static_cast<size_t>(q.first_row + token) * c.q_row_stride +
-                              (static_cast<size_t>(head) * p.group + (pair - token * p.group)) * c.q_head_stride;
+            const int32_t pair = pair0 + tile * kTileRows + row0 + (s0 + i) * kAtOnce + lane / kLanes;
+            const int32_t token = pair / static_cast<int32_t>(p.group);
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (pair < rows) {
+              const uint16_t *at = static_cast<const uint16_t *>(c.q) + static_cast<size_t>(q.first_row + token) * c.q_row_stride +
+                                   (static_cast<size_t>(head) * p.group + (pair - token * p.group)) * c.q_head_stride + 8 * sub;
+              if (vector) {
+                raw[i] = *reinterpret_cast<const uint4 *>(at);
+              } else {
+                uint32_t w[4];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              x[i][b] = pair < rows ? load_typed(c.q, at + b * 32 + lane, c.type) : 0.0f;
+                for (int e = 0; e < 4; ++e)
+                  w[e] = at[2 * e] | static_cast<uint32_t>(at[2 * e + 1]) << 16;
+                raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
           }
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
-            float top = 0.0f;
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[8], top = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              top = fmaxf(top, fabsf(x[i][b]));
+            for (int e = 0; e < 4; ++e) {
+              if (c.type == TCRV_CUDA_TYPE_F16) {
+                const float2 f = __half22float2(bits_half2(w[e]));
+                x[2 * e] = f.x, x[2 * e + 1] = f.y;
+              } else {
+                x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+              }
+              top = fmaxf(top, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
+            }
 #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1)
+            for (int off = kLanes / 2; off >= 1; off >>= 1)
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            int k = 0;
-            if (top > 0.0f && top < INFINITY)
-              k = min(120, 14 - ilogbf(top));
-            const float lift = exp2f(static_cast<float>(k)) * (c.scale < 0.0f ? -1.0f : 1.0f);
-            const int row = row0 + i0 + i;
-            if (lane == i0 + i)
-              my_lift = k;
+            const int k = top > 0.0f && top < INFINITY ? min(120, 141 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
+            const float lift = __uint_as_float(static_cast<uint32_t>(127 + k) << 23) * sign;
+            const int in_warp = (s0 + i) * kAtOnce + lane / kLanes, row = row0 + in_warp;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              const int chunk = 2 * t + (b & 1);
-              *reinterpret_cast<__half *>(operand + (b >> 1) * L::kPanel + row * 128 + ((chunk ^ (row & 7)) << 4) + f * 2) =
-                  __float2half_rn(x[i][b] * lift);
+            for (int h = 0; h < kAtOnce; ++h) {  // lane `row` keeps the row's power
+              const int its = __shfl_sync(0xffffffffu, k, h * kLanes);
+              if (lane == (s0 + i) * kAtOnce + h)
+                my_lift = its;
+            }
+            uint8_t *line = operand + (b >> 1) * L::kPanel + row * 128 + high * 8;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // elements 4t', 4t'+2, 4t'+1, 4t'+3 of the half block
+              const int chunk = 2 * (t + u) + (b & 1);
+              const uint2 v = make_uint2(half2_bits(__floats2half2_rn(x[4 * u] * lift, x[4 * u + 2] * lift)),
+                                         half2_bits(__floats2half2_rn(x[4 * u + 1] * lift, x[4 * u + 3] * lift)));
+              *reinterpret_cast<uint2 *>(line + ((chunk ^ (row & 7)) << 4)) = v;
             }
           }
         }
@@ -255,7 +318,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       }
       const int32_t pair = pair0 + tile * kTileRows + row0 + lane, token = pair / static_cast<int32_t>(p.group);
       const int32_t position = pair < rows ? before + token : -1;
-      const float scale = fabsf(c.scale) * kLog2e * exp2f(static_cast<float>(-my_lift));
+      const float scale = fabsf(c.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - my_lift) << 23);
       const uint32_t scores = tmem + quadrant + tile * 128, sums = tmem + quadrant + 256 + tile * kDim;
       const int32_t tile_pair0 = pair0 + tile * kTileRows;
       const int32_t tile_from = window ? before + (min(rows, tile_pair0 + kTileRows) - 1) / static_cast<int32_t>(p.group) - window + 1 : 0;
@@ -278,22 +341,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           s *= scale * ((flag & 2u) ? 16.0f : 1.0f);
           return (flag & 1u) && at <= position && !(window && at <= position - window) ? s : -INFINITY;
         };
-        float top = -INFINITY;
+        uint32_t s[2][32];  // a chunk is on its way while the one before is worked on
+        tmem_ld_32x32b<32>(scores, s[0]);
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
-          uint32_t s[32];
-          tmem_ld_32x32b<32>(scores + ch * 32, s);
           tmem_ld_wait();
+          tmem_ld_32x32b<32>(scores + (ch + 1) % 4 * 32, s[(ch + 1) & 1]);
           if (whole) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              top = fmaxf(top, __uint_as_float(s[i]));
+            for (int i = 0; i < 32; i += 2)
+              tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], __uint_as_float(s[ch & 1][i]), __uint_as_float(s[ch & 1][i + 1]));
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              top = fmaxf(top, masked(__uint_as_float(s[i]), ch * 32 + i));
+              tops[i & 3] = fmaxf(tops[i & 3], masked(__uint_as_float(s[ch & 1][i]), ch * 32 + i));
           }
         }
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         if (whole)
           top *= scale;
         const bool grown = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
@@ -318,35 +383,41 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;
+        float2 parts[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
-          uint32_t s[32], w[16];
-          tmem_ld_32x32b<32>(scores + ch * 32, s);
+          uint32_t w[16];
           tmem_ld_wait();
+          if (ch < 3)
+            tmem_ld_32x32b<32>(scores + (ch + 1) * 32, s[(ch + 1) & 1]);
+          const uint32_t(&v)[32] = s[ch & 1];
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float a = exp2_fast(fmaf(__uint_as_float(s[i]), scale, -base));
-              const float b = exp2_fast(fmaf(__uint_as_float(s[i + 1]), scale, -base));
-              l += a + b;
-              w[i / 2] = half2_bits(__floats2half2_rn(a, b));
+              float2 x = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, base2);
+              x.x = exp2_fast(x.x);
+              x.y = exp2_fast(x.y);
+              parts[(i >> 1) & 1] = add2(parts[(i >> 1) & 1], x);
+              w[i / 2] = half2_bits(__floats2half2_rn(x.x, x.y));
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float a = exp2_fast(masked(__uint_as_float(s[i]), ch * 32 + i) - base);
-              float b = exp2_fast(masked(__uint_as_float(s[i + 1]), ch * 32 + i + 1) - base);
-              l += a + b;
+              float2 x = make_float2(exp2_fast(masked(__uint_as_float(v[i]), ch * 32 + i) - base),
+                                     exp2_fast(masked(__uint_as_float(v[i + 1]), ch * 32 + i + 1) - base));
+              parts[(i >> 1) & 1] = add2(parts[(i >> 1) & 1], x);
               const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * ((ch * 32 + i) / kGroupTokens))) & 0xffu;
               if (flag & 4u) {
-                a *= 16.0f;
-                b *= 16.0f;
+                x.x *= 16.0f;
+                x.y *= 16.0f;
               }
-              w[i / 2] = half2_bits(__floats2half2_rn(a, b));
+              w[i / 2] = half2_bits(__floats2half2_rn(x.x, x.y));
             }
           }
           tmem_st_32x32b_x16(scores + ch * 16, w);
         }
+        l += (parts[0].x + parts[0].y) + (parts[1].x + parts[1].y);
         if (group_flags & 0x0808080808080808ull) {  // a value that is no number: the rows that see its token are none either
           for (int i = 0; i < kTileTokens; ++i) {
             const int32_t at = token0 + i;
@@ -424,32 +495,40 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
               l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < kProductWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQuantRegs));
     // ================================================================ quants -> fp16 operands
+    // a warp to each group of a tile
     const int w = warp - 8, g = lane >> 2, t = lane & 3;
-    const uint32_t per_page = static_cast<uint32_t>(c.cache.groups);
+    const int32_t per_page = static_cast<int32_t>(c.cache.groups);
     const int32_t groups = (q.len + kGroupTokens - 1) / kGroupTokens;
     const int32_t *table = c.block_table + r * c.table_stride;
-    // group i (0 or 1) of this warp in tile j
-    const auto group_of = [&](int j, int i) { return (tile_begin + j) * kTileGroups + w + 4 * i; };
-    const auto page_of = [&](int j, int i) -> int32_t {
-      const int32_t at = group_of(j, i);
-      return j < tiles && at < groups ? table[static_cast<uint32_t>(at) / per_page] : -1;
+    // the group whose page is asked for next, and its place in its page
+    int32_t at = tile_begin * kTileGroups + w, page_at = at / per_page, in_page = at - page_at * per_page, page = -1, place = 0;
+    const int32_t end = min(groups, tile_end * kTileGroups);
+    const auto ask = [&]() {
+      page = at < end ? table[page_at] : -1;
+      place = in_page;
+      at += kTileGroups;
+      in_page += kTileGroups;
+      while (in_page >= per_page) {
+        in_page -= per_page;
+        ++page_at;
+      }
     };
-    const auto fetch = [&](RawGroup<NB> &raw, int j, int i, int32_t page) {
+    const auto fetch = [&](RawGroup<NB> &raw) {
       raw.there = page >= 0 && static_cast<size_t>(page) < c.cache.pages;
       if (raw.there) {
-        const uint32_t in_page = static_cast<uint32_t>(group_of(j, i)) % per_page;
-        const uint8_t *at = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
-                            (static_cast<size_t>(head) * per_page + in_page) * (18 * kDim);
-        load_global<NB>(raw.key[0], at + lane * NB * 4);
-        load_global<NB>(raw.key[1], at + 128 * NB + lane * NB * 4);
-        load_global<NB>(raw.value[0], at + 256 * NB + lane * NB * 4);
-        load_global<NB>(raw.value[1], at + 384 * NB + lane * NB * 4);
-        load_global<NB / 2>(raw.key_scale[0], at + 512 * NB + g * NB * 2);
-        load_global<NB / 2>(raw.key_scale[1], at + 512 * NB + (g + 8) * NB * 2);
-        load_global<NB>(raw.value_scale[0], at + 544 * NB + 2 * t * NB * 2);
-        load_global<NB>(raw.value_scale[1], at + 544 * NB + (2 * t + 8) * NB * 2);
+        const uint8_t *from = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
+                              (static_cast<size_t>(head) * per_page + place) * (18 * kDim);
+        load_global<NB>(raw.key[0], from + lane * NB * 4);
+        load_global<NB>(raw.key[1], from + 128 * NB + lane * NB * 4);
+        load_global<NB>(raw.value[0], from + 256 * NB + lane * NB * 4);
+        load_global<NB>(raw.value[1], from + 384 * NB + lane * NB * 4);
+        load_global<NB / 2>(raw.key_scale[0], from + 512 * NB + g * NB * 2);
+        load_global<NB / 2>(raw.key_scale[1], from + 512 * NB + (g + 8) * NB * 2);
+        load_global<NB>(raw.value_scale[0], from + 544 * NB + 2 * t * NB * 2);
+        load_global<NB>(raw.value_scale[1], from + 544 * NB + (2 * t + 8) * NB * 2);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -462,101 +541,95 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         }
       }
     };
-    const auto half_of = [](const uint32_t *words, int i) -> uint32_t { return (words[i >> 1] >> (16 * (i & 1))) & 0xffffu; };
-    RawGroup<NB> now[2], ahead[2];
-    int32_t pages[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      fetch(ahead[i], 0, i, page_of(0, i));
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      pages[i] = page_of(1, i);
+    RawGroup<NB> now, ahead;
+    ask();
+    fetch(ahead);
+    ask();
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
       const int stage = j & 1, slot = j % kSlots;
+      now = ahead;
+      fetch(ahead);
+      ask();
+      // ---- scales: of values, two tokens side by side; none for tokens behind the context; large ones are seen to
+      const int32_t left = q.len - ((tile_begin + j) * kTileGroups + w) * kGroupTokens;
+      uint32_t large_key = 0, large_value = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        now[i] = ahead[i];
-        fetch(ahead[i], j + 1, i, pages[i]);
-        pages[i] = page_of(j + 2, i);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pair[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          pair[b] = __byte_perm(now.value_scale[h][b / 2], now.value_scale[h][NB / 2 + b / 2], (b & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          now.value_scale[h][b] = pair[b];
+      }
+      if (left < kGroupTokens) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t keep = (2 * t + 8 * h < left ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < left ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            now.value_scale[h][b] &= keep;
+#pragma unroll
+          for (int b = 0; b < NB / 2; ++b)
+            now.key_scale[h][b] = g + 8 * h < left ? now.key_scale[h][b] : 0;
+        }
+      }
+      // |d| >= 2^13, with infinities and NaN: 8 d may leave fp16
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 0; b < NB / 2; ++b)
+          large_key |= (now.key_scale[h][b] & 0x7fff7fffu) + 0x10001000u;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          large_value |= (now.value_scale[h][b] & 0x7fff7fffu) + 0x10001000u;
+      }
+      uint32_t flag = now.there ? 1u : 0u;
+      if (__any_sync(0xffffffffu, ((large_key | large_value) & 0x80008000u) != 0)) {
+        const __half2 sixteenth = __float2half2_rn(0.0625f);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < NB / 2; ++b)
+            now.key_scale[h][b] = half2_bits(__hmul2(bits_half2(now.key_scale[h][b]), sixteenth));
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            if ((now.value_scale[h][b] & 0x7c00u) == 0x7c00u) {
+              bad |= 1u << (2 * t + 8 * h);
+              now.value_scale[h][b] &= 0xffff0000u;
+            }
+            if ((now.value_scale[h][b] & 0x7c000000u) == 0x7c000000u) {
+              bad |= 2u << (2 * t + 8 * h);
+              now.value_scale[h][b] &= 0xffffu;
+            }
+            now.value_scale[h][b] = half2_bits(__hmul2(bits_half2(now.value_scale[h][b]), sixteenth));
+          }
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        flag |= bad ? 14u : 6u;
+        if (lane == 0)
+          poison[slot * kTileGroups + w] = static_cast<uint16_t>(bad);
       }
       if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
         break;
-      // ---- scales: none for tokens behind the context, the others checked
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int32_t first = group_of(j, i) * kGroupTokens, left = q.len - first;
-        uint32_t big_key = 0, big_value = 0, bad = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (g + 8 * h >= left) {
-#pragma unroll
-            for (int b = 0; b < NB / 2; ++b)
-              now[i].key_scale[h][b] = 0;
-          }
-          uint32_t keep = (2 * t + 8 * h < left ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < left ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int b = 0; b < NB / 2; ++b)
-            big_key |= ((now[i].key_scale[h][b] & 0x7fff7fffu) + 0x10001000u) & 0x80008000u;  // |d| >= 2^13: 8 d leaves fp16
-          // pairs of tokens side by side
-          uint32_t pair[NB];
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            pair[b] = (half_of(now[i].value_scale[h], b) | (half_of(now[i].value_scale[h], NB + b) << 16)) & keep;
-            const uint32_t size = pair[b] & 0x7fff7fffu;
-            if ((size & 0x7c00u) == 0x7c00u) {
-              bad |= 1u << (2 * t + 8 * h);
-              pair[b] &= 0xffff0000u;
-            }
-            if ((size & 0x7c000000u) == 0x7c000000u) {
-              bad |= 2u << (2 * t + 8 * h);
-              pair[b] &= 0xffffu;
-            }
-            big_value |= ((pair[b] & 0x7fff7fffu) + 0x10001000u) & 0x80008000u;
-          }
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            now[i].value_scale[h][b] = pair[b];
-        }
-        const bool some_key = __any_sync(0xffffffffu, big_key != 0), some_value = __any_sync(0xffffffffu, big_value != 0);
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        if (lane == 0) {
-          flags[slot * kTileGroups + w + 4 * i] =
-              static_cast<uint8_t>((now[i].there ? 1 : 0) | (some_key ? 2 : 0) | (some_value ? 4 : 0) | (bad ? 8 : 0));
-          poison[slot * kTileGroups + w + 4 * i] = static_cast<uint16_t>(bad);
-        }
-        if (some_key || some_value) {
-          const __half2 sixteenth = __float2half2_rn(0.0625f);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int b = 0; b < NB / 2; ++b)
-              if (some_key)
-                now[i].key_scale[h][b] = half2_bits(__hmul2(bits_half2(now[i].key_scale[h][b]), sixteenth));
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-              if (some_value)
-                now[i].value_scale[h][b] = half2_bits(__hmul2(bits_half2(now[i].value_scale[h][b]), sixteenth));
-          }
-        }
-      }
+      if (lane == 0)
+        flags[slot * kTileGroups + w] = static_cast<uint8_t>(flag);
       // ---- keys: a word's 8 elements are 16 bytes of the token's row; neighbouring lanes' chunks fall on different banks
-      uint8_t *keys = smem + L::kKey + stage * L::kKeyBytes;
+      uint8_t *keys = smem + L::kKey + stage * L::kKeyBytes + (w * kGroupTokens + g) * 128;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = (w + 4 * i) * kGroupTokens + h * 8 + g;
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const uint32_t word = now[i].key[h][b], d = half_of(now[i].key_scale[h], b);
-            const __half2 scale = bits_half2(d | (d << 16));
-            const uint4 v = make_uint4(half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
-                                       half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
-                                       half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
-                                       half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale)));
-            *reinterpret_cast<uint4 *>(keys + (b >> 1) * L::kPanel + row * 128 + (((2 * t + (b & 1)) ^ (row & 7)) << 4)) = v;
-          }
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t word = now.key[h][b];
+          const __half2 scale = bits_half2(__byte_perm(now.key_scale[h][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
+          const uint4 v = make_uint4(half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
+                                     half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
+                                     half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
+                                     half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale)));
+          *reinterpret_cast<uint4 *>(keys + (b >> 1) * L::kPanel + h * 1024 + (((2 * t + (b & 1)) ^ g) << 4)) = v;
         }
       }
       fence_proxy_async();
@@ -566,26 +639,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       // ---- values, transposed: row n of the operand is an element, its columns the tokens
       if (j >= 2 && !wait(kBarValueFree + stage, (j >> 1) - 1))
         break;
-      uint8_t *values = smem + L::kValue + stage * L::kValueBytes;
+      uint8_t *values = smem + L::kValue + stage * L::kValueBytes + (w >> 2) * (kDim * 128) + g * 128 + t * 4;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int group = w + 4 * i;
+      for (int h = 0; h < 2; ++h) {
+        uint8_t *column = values + ((((w & 3) * 2 + h) ^ g) << 4);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int chunk = (group & 3) * 2 + h;
-          uint8_t *panel = values + (group >> 2) * (kDim * 128) + ((chunk ^ g) << 4) + t * 4;
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t word = now.value[h][b];
+          const __half2 scale = bits_half2(now.value_scale[h][b]);
+          const uint32_t v[4] = {half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
+                                 half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
+                                 half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
+                                 half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale))};
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const uint32_t word = now[i].value[h][b];
-            const __half2 scale = bits_half2(now[i].value_scale[h][b]);
-            const uint32_t v[4] = {half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
-                                   half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
-                                   half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
-                                   half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale))};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint32_t *>(panel + ((b * 4 + k) * 8 + g) * 128) = v[k];
-          }
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint32_t *>(column + (b * 4 + k) * 1024) = v[k];
         }
       }
       fence_proxy_async();
@@ -593,7 +661,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       if (lane == 0)
         mbar_arrive(&bars[kBarValueFull + stage]);
     }
-  } else if (tiles > 0) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegs));
+    if (warp == kProductWarp && tiles > 0) {
     // ================================================================ products: one lane issues
     const uint32_t base = smem_addr(smem);
     constexpr uint32_t kScoreDesc = umma_idesc_f16(kTileRows, kTileTokens), kSumDesc = umma_idesc_f16(kTileRows, kDim);
@@ -646,12 +716,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         __syncwarp();
       }
     }
+    }
   }
   // ---- the tensor memory goes back when every role is through with it
   tcgen05_fence_before_thread_sync();
   __syncthreads();
   tcgen05_fence_after_thread_sync();
-  if (warp == 12)
+  if (warp == kProductWarp)
     tmem_dealloc(tmem, 512);
 }
 
