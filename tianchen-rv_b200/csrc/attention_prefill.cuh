@@ -4,7 +4,7 @@
 // A CTA takes 256 rows, two tiles of 128 (row = new token * heads of the kv head + head, so the heads that share a
 // cache head share its tiles), and walks over the context in tiles of 128 tokens:
 //   S = Q K^T (128 x 128, f32, TMEM)  ->  P = 2^(S * scale - m) (fp16, TMEM, over S)  ->  O += P V (128 x D, f32, TMEM).
-// Warps 0..3 and 4..7 are the soft-max of the two tiles, a thread to a row; warps 8..15 turn quants into the fp16
+// Warps 0..7 are the soft-max, of one tile after the other: two threads to a row, 64 columns each; warps 8..15 turn quants into the fp16
 // operands in shared memory, warp 16 issues the products.  While one tile's soft-max runs the other tile's products do.
 //
 // Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
@@ -13,6 +13,8 @@
 // its values leave fp16 is held at 1/16 and made good in S or in P.  The running maximum that P is relative to follows the
 // true one only when that has grown by more than 2^8: then O is rescaled, otherwise P just has values up to 2^8.
 #pragma once
+
+#include <type_traits>
 
 #include "attention_columns.cuh"
 #include "tcgen05.cuh"
@@ -58,35 +60,45 @@ struct PrefillLayout {
   static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
   static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group]: tokens with a value scale that is no number
   static constexpr int kBars = kPoison + kSlots * kTileGroups * 2;
-  static constexpr int kBarCount = 15;
-  static constexpr int kTmem = kBars + kBarCount * 8;
+  static constexpr int kBarCount = 19;
+  static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
+  static constexpr int kTmem = kTops + 2 * 2 * 128 * 4;
   static constexpr int kAbort = kTmem + 4;
   static constexpr int kBytes = kAbort + 4 + 1024;  // (the base is rounded up to 1024)
 };
 
 // barriers
-enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13 };
+enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15 };
 
 // kind::f16, fp16 A and B (both K-major), f32 D.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// The upper half of umma_desc_k_major_sw128's descriptor does not depend on the address.
+constexpr uint32_t kDescHigh = static_cast<uint32_t>((static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61) >> 32);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_byte_addr) { return ((smem_byte_addr & 0x3ffffu) >> 4) | (1u << 16); }
+template <bool kAdd>
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %4};\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "n"(kAdd ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      ".reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "r"(add)
       : "memory");
 }
 
@@ -204,16 +216,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   const int tiles = tile_end - tile_begin;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars[kBarQuery], 4 * tiles_q);
+    mbar_init(&bars[kBarQuery], 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[kBarKeyFull + i], kQuantWarps);
       mbar_init(&bars[kBarKeyFree + i], 1);
       mbar_init(&bars[kBarValueFull + i], kQuantWarps);
       mbar_init(&bars[kBarValueFree + i], 1);
       mbar_init(&bars[kBarScores + i], 1);
-      mbar_init(&bars[kBarWeights + i], 4);
+      mbar_init(&bars[kBarWeights + i], 8);
       mbar_init(&bars[kBarSums + i], 1);
     }
+    for (int i = 0; i < 4; ++i)
+      mbar_init(&bars[kBarPair + i], 2);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -239,228 +253,270 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    // ================================================================ soft-max of one tile
-    const int tile = warp >> 2;
-    if (tile < tiles_q) {
-      // ---- the query operand: this warp's 32 rows, in the key operand's order of elements, and a power of two that lifts
-      // the largest element into [2^14, 2^15).  kDim / 8 lanes to a row, eight elements to a lane.
-      const int row0 = (warp & 3) * 32;
-      const uint32_t quadrant = static_cast<uint32_t>(row0) << 16;
+    // ================================================================ soft-max of both tiles in turn
+    // Two threads to a row, lane quadrant `warp & 3` and columns 64 * half .. + 63: the two warps of a scheduler then keep its
+    // exponential unit busy together, and one tile's products run while the other tile's weights are made.
+    const int half = warp >> 2, row0 = (warp & 3) * 32, row = row0 + lane;
+    const uint32_t quadrant = static_cast<uint32_t>(row0) << 16;
+    const int32_t group = static_cast<int32_t>(p.group);
+    float *tops = reinterpret_cast<float *>(smem + L::kTops);
+    int lifts = 0;  // powers of the queries of this thread's row in the two tiles, a byte each
+    {
+      // ---- the query operand, tile `half`: 32 rows of it, in the key operand's order of elements, times a power of two that
+      // lifts the largest element into [2^14, 2^15).  kDim / 8 lanes to a row, eight elements to a lane.
+      constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = 8;
+      uint8_t *operand = smem + L::kQuery + half * L::kKeyBytes;
+      const int sub = lane % kLanes, b = sub >> 2, high = (sub >> 1) & 1, t = (sub & 1) * 2;
+      const bool vector = (reinterpret_cast<uintptr_t>(c.q) & 15u) == 0 && ((c.q_row_stride | c.q_head_stride) & 7u) == 0;
+      const float sign = c.scale < 0.0f ? -1.0f : 1.0f;
       int my_lift = 0;
-      {
-        constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = 8;
-        uint8_t *operand = smem + L::kQuery + tile * L::kKeyBytes;
-        const int sub = lane % kLanes, b = sub >> 2, high = (sub >> 1) & 1, t = (sub & 1) * 2;
-        const bool vector = (reinterpret_cast<uintptr_t>(c.q) & 15u) == 0 && ((c.q_row_stride | c.q_head_stride) & 7u) == 0;
-        const float sign = c.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll 1
-        for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
-          uint4 raw[kBatch];
+      for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+        uint4 raw[kBatch];
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int32_t pair = pair0 + tile * kTileRows + row0 + (s0 + i) * kAtOnce + lane / kLanes;
-            const int32_t token = pair / static_cast<int32_t>(p.group);
-            raw[i] = make_uint4(0, 0, 0, 0);
-            if (pair < rows) {
-              const uint16_t *at = static_cast<const uint16_t *>(c.q) + static_cast<size_t>(q.first_row + token) * c.q_row_stride +
-                                   (static_cast<size_t>(head) * p.group + (pair - token * p.group)) * c.q_head_stride + 8 * sub;
-              if (vector) {
-                raw[i] = *reinterpret_cast<const uint4 *>(at);
-              } else {
-                uint32_t w[4];
+        for (int i = 0; i < kBatch; ++i) {
+          const int32_t pair = pair0 + half * kTileRows + row0 + (s0 + i) * kAtOnce + lane / kLanes, token = pair / group;
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (pair < rows) {
+            const uint16_t *at = static_cast<const uint16_t *>(c.q) + static_cast<size_t>(q.first_row + token) * c.q_row_stride +
+                                 (static_cast<size_t>(head) * group + (pair - token * group)) * c.q_head_stride + 8 * sub;
+            if (vector) {
+              raw[i] = *reinterpret_cast<const uint4 *>(at);
+            } else {
+              uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  w[e] = at[2 * e] | static_cast<uint32_t>(at[2 * e + 1]) << 16;
-                raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-            float x[8], top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (c.type == TCRV_CUDA_TYPE_F16) {
-                const float2 f = __half22float2(bits_half2(w[e]));
-                x[2 * e] = f.x, x[2 * e + 1] = f.y;
-              } else {
-                x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-              }
-              top = fmaxf(top, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
-            }
-#pragma unroll
-            for (int off = kLanes / 2; off >= 1; off >>= 1)
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const int k = top > 0.0f && top < INFINITY ? min(120, 141 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
-            const float lift = __uint_as_float(static_cast<uint32_t>(127 + k) << 23) * sign;
-            const int in_warp = (s0 + i) * kAtOnce + lane / kLanes, row = row0 + in_warp;
-#pragma unroll
-            for (int h = 0; h < kAtOnce; ++h) {  // lane `row` keeps the row's power
-              const int its = __shfl_sync(0xffffffffu, k, h * kLanes);
-              if (lane == (s0 + i) * kAtOnce + h)
-                my_lift = its;
-            }
-            uint8_t *line = operand + (b >> 1) * L::kPanel + row * 128 + high * 8;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {  // elements 4t', 4t'+2, 4t'+1, 4t'+3 of the half block
-              const int chunk = 2 * (t + u) + (b & 1);
-              const uint2 v = make_uint2(half2_bits(__floats2half2_rn(x[4 * u] * lift, x[4 * u + 2] * lift)),
-                                         half2_bits(__floats2half2_rn(x[4 * u + 1] * lift, x[4 * u + 3] * lift)));
-              *reinterpret_cast<uint2 *>(line + ((chunk ^ (row & 7)) << 4)) = v;
+              for (int e = 0; e < 4; ++e)
+                w[e] = at[2 * e] | static_cast<uint32_t>(at[2 * e + 1]) << 16;
+              raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&bars[kBarQuery]);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          float x[8], top = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (c.type == TCRV_CUDA_TYPE_F16) {
+              const float2 f = __half22float2(bits_half2(w[e]));
+              x[2 * e] = f.x, x[2 * e + 1] = f.y;
+            } else {
+              x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+            top = fmaxf(top, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
+          }
+#pragma unroll
+          for (int off = kLanes / 2; off >= 1; off >>= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const int k = top > 0.0f && top < INFINITY ? min(120, 141 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
+          const float lift = __uint_as_float(static_cast<uint32_t>(127 + k) << 23) * sign;
+          const int line_row = row0 + (s0 + i) * kAtOnce + lane / kLanes;
+#pragma unroll
+          for (int h = 0; h < kAtOnce; ++h) {  // lane `row` keeps the row's power
+            const int its = __shfl_sync(0xffffffffu, k, h * kLanes);
+            if (lane == (s0 + i) * kAtOnce + h)
+              my_lift = its;
+          }
+          uint8_t *line = operand + (b >> 1) * L::kPanel + line_row * 128 + high * 8;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {  // elements 4t', 4t'+2, 4t'+1, 4t'+3 of the half block
+            const int chunk = 2 * (t + u) + (b & 1);
+            const uint2 v = make_uint2(half2_bits(__floats2half2_rn(x[4 * u] * lift, x[4 * u + 2] * lift)),
+                                       half2_bits(__floats2half2_rn(x[4 * u + 1] * lift, x[4 * u + 3] * lift)));
+            *reinterpret_cast<uint2 *>(line + ((chunk ^ (line_row & 7)) << 4)) = v;
+          }
+        }
       }
-      const int32_t pair = pair0 + tile * kTileRows + row0 + lane, token = pair / static_cast<int32_t>(p.group);
-      const int32_t position = pair < rows ? before + token : -1;
-      const float scale = fabsf(c.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - my_lift) << 23);
+      // the row's power in the other tile is the other warp's
+      reinterpret_cast<int *>(tops)[half * 128 + row] = my_lift;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars[kBarQuery]);
+        mbar_arrive(&bars[kBarPair + (warp & 3)]);
+      }
+      if (wait(kBarPair + (warp & 3), 0)) {
+        const int other = reinterpret_cast<int *>(tops)[(1 - half) * 128 + row];
+        lifts = half == 0 ? (my_lift & 0xff) | other << 8 : (other & 0xff) | my_lift << 8;
+      }
+    }
+    // what changes between the tiles; the loop below swaps `mine` and `other` after each step
+    struct State {
+      float m, l, scale;
+      int32_t position, from, to;  // what this row sees up to; tokens that all rows of the tile see
+    };
+    const auto state_of = [&](int tile, int lift) {
+      const int32_t pair = pair0 + tile * kTileRows + row;
+      State st;
+      st.position = pair < rows ? before + pair / group : -1;
+      // (a row that sees nothing has a maximum, so that it does not hold up its warp)
+      st.m = st.position < 0 ? 0.0f : -INFINITY;
+      st.l = 0.0f;
+      st.scale = fabsf(c.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - lift) << 23);
+      const int32_t first = pair0 + tile * kTileRows;
+      st.from = window ? before + (min(rows, first + kTileRows) - 1) / group - window + 1 : 0;
+      st.to = before + first / group - (kTileTokens - 1);
+      return st;
+    };
+    State mine = state_of(0, static_cast<int8_t>(lifts)), other = state_of(1, static_cast<int8_t>(lifts >> 8));
+    const int steps = tiles * tiles_q;
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const int tile = tiles_q == 2 ? step & 1 : 0, j = tiles_q == 2 ? step >> 1 : step;
+      if (!wait(kBarScores + tile, j))
+        break;
+      tcgen05_fence_after_thread_sync();
       const uint32_t scores = tmem + quadrant + tile * 128, sums = tmem + quadrant + 256 + tile * kDim;
-      const int32_t tile_pair0 = pair0 + tile * kTileRows;
-      const int32_t tile_from = window ? before + (min(rows, tile_pair0 + kTileRows) - 1) / static_cast<int32_t>(p.group) - window + 1 : 0;
-      const int32_t tile_to = before + tile_pair0 / static_cast<int32_t>(p.group);
-      float m = -INFINITY, l = 0.0f;
-      bool going = true;
-#pragma unroll 1
-      for (int j = 0; j < tiles && going; ++j) {
-        if (!wait(kBarScores + tile, j))
-          break;
-        tcgen05_fence_after_thread_sync();
-        const int32_t token0 = (tile_begin + j) * kTileTokens;
-        const int slot = j % kSlots;
-        const uint64_t group_flags = *reinterpret_cast<volatile uint64_t *>(smem + L::kFlags + slot * kTileGroups);
-        const bool whole = group_flags == 0x0101010101010101ull && token0 >= tile_from && token0 + kTileTokens - 1 <= tile_to;
-        // what a score counts as, with the mask and the groups' flags
-        const auto masked = [&](float s, int column) {
-          const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (column / kGroupTokens))) & 0xffu;
-          const int32_t at = token0 + column;
-          s *= scale * ((flag & 2u) ? 16.0f : 1.0f);
-          return (flag & 1u) && at <= position && !(window && at <= position - window) ? s : -INFINITY;
-        };
-        uint32_t s[2][32];  // a chunk is on its way while the one before is worked on
-        tmem_ld_32x32b<32>(scores, s[0]);
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t s[64], w[32];
+      tmem_ld_32x32b<32>(scores + half * 64, *reinterpret_cast<uint32_t(*)[32]>(s));
+      tmem_ld_32x32b<32>(scores + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+      const int32_t token0 = (tile_begin + j) * kTileTokens;
+      const int slot = j % kSlots;
+      const uint64_t group_flags = *reinterpret_cast<volatile uint64_t *>(smem + L::kFlags + slot * kTileGroups);
+      const bool whole = group_flags == 0x0101010101010101ull && token0 >= mine.from && token0 <= mine.to;
+      // columns that this row sees
+      const int32_t upper = mine.position - token0 - half * 64, lower = window ? upper - window + 1 : 0;
+      if (!whole) {  // scores in powers of two, unseen ones -infinity; the weights' scale is 1 then
+        tmem_ld_wait();
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          tmem_ld_wait();
-          tmem_ld_32x32b<32>(scores + (ch + 1) % 4 * 32, s[(ch + 1) & 1]);
-          if (whole) {
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (4 * half + h)));
+          const float by = (flag & 2u) ? 16.0f * mine.scale : mine.scale;
+          const int32_t to = (flag & 1u) ? upper : -1;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], __uint_as_float(s[ch & 1][i]), __uint_as_float(s[ch & 1][i + 1]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              tops[i & 3] = fmaxf(tops[i & 3], masked(__uint_as_float(s[ch & 1][i]), ch * 32 + i));
-          }
+          for (int i = 16 * h; i < 16 * h + 16; ++i)
+            s[i] = i <= to && i >= lower ? __float_as_uint(__uint_as_float(s[i]) * by) : 0xff800000u;
         }
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        if (whole)
-          top *= scale;
-        const bool grown = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
-        if (__any_sync(0xffffffffu, grown)) {
-          const float now = grown ? top : m, alpha = grown ? exp2_fast(m - now) : 1.0f;
-          m = now;
-          l *= alpha;
-          if (j > 0) {
-            if (!wait(kBarSums + tile, j - 1))
-              break;
-            tcgen05_fence_after_thread_sync();
-#pragma unroll
-            for (int ch = 0; ch < kDim / 16; ++ch) {
-              uint32_t o[16];
-              tmem_ld_32x32b<16>(sums + ch * 16, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x32b_x16(sums + ch * 16, o);
-            }
-          }
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        float2 parts[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint32_t w[16];
-          tmem_ld_wait();
-          if (ch < 3)
-            tmem_ld_32x32b<32>(scores + (ch + 1) * 32, s[(ch + 1) & 1]);
-          const uint32_t(&v)[32] = s[ch & 1];
-          if (whole) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 x = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, base2);
-              x.x = exp2_fast(x.x);
-              x.y = exp2_fast(x.y);
-              parts[(i >> 1) & 1] = add2(parts[(i >> 1) & 1], x);
-              w[i / 2] = half2_bits(__floats2half2_rn(x.x, x.y));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 x = make_float2(exp2_fast(masked(__uint_as_float(v[i]), ch * 32 + i) - base),
-                                     exp2_fast(masked(__uint_as_float(v[i + 1]), ch * 32 + i + 1) - base));
-              parts[(i >> 1) & 1] = add2(parts[(i >> 1) & 1], x);
-              const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * ((ch * 32 + i) / kGroupTokens))) & 0xffu;
-              if (flag & 4u) {
-                x.x *= 16.0f;
-                x.y *= 16.0f;
-              }
-              w[i / 2] = half2_bits(__floats2half2_rn(x.x, x.y));
-            }
-          }
-          tmem_st_32x32b_x16(scores + ch * 16, w);
-        }
-        l += (parts[0].x + parts[0].y) + (parts[1].x + parts[1].y);
-        if (group_flags & 0x0808080808080808ull) {  // a value that is no number: the rows that see its token are none either
-          for (int i = 0; i < kTileTokens; ++i) {
-            const int32_t at = token0 + i;
-            if (((poison[slot * kTileGroups + i / kGroupTokens] >> (i % kGroupTokens)) & 1) && at <= position && !(window && at <= position - window))
-              l = NAN;
-          }
-        }
-        tmem_st_wait();
-        tcgen05_fence_before_thread_sync();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&bars[kBarWeights + tile]);
       }
-      // ---- the row's result; element n of the sums is d = 32 (n / 32) + 16 ((n >> 4) & 1) + 2 (n & 7) + ((n >> 3) & 1)
+      const float by = whole ? mine.scale : 1.0f;
+      // Weights relative to the maximum of the tiles before, which is as good as this tile's own unless that is more than 2^8
+      // above it (or there is none yet): then the accumulators are rescaled and the weights made again.
+      tmem_ld_wait();
+      float top;
+      {
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2)
+          most[(i >> 1) & 3] = max3(most[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * by;
+      }
+      // to the thread that has the row's other half; its maximum is here by the time the weights are made
+      float *exchange = tops + ((step + 1) & 1) * 256;  // (the prologue's was the first)
+      exchange[half * 128 + row] = top;
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars[kBarPair + (warp & 3)]);
+      float2 parts[2];
+      const auto weigh = [&](float base) {
+        const float2 by2 = make_float2(by, by), base2 = make_float2(-base, -base);
+        parts[0] = parts[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          float2 x = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), by2, base2);
+          x.x = exp2_fast(x.x);
+          x.y = exp2_fast(x.y);
+          parts[(i >> 1) & 1] = add2(parts[(i >> 1) & 1], x);
+          w[i / 2] = half2_bits(__floats2half2_rn(x.x, x.y));
+        }
+      };
+      if (j > 0)
+        weigh(mine.m == -INFINITY ? 0.0f : mine.m);
+      if (!wait(kBarPair + (warp & 3), step + 1))
+        break;
+      top = fmaxf(top, exchange[(1 - half) * 128 + row]);
+      const bool grown = top > mine.m + 8.0f || (mine.m == -INFINITY && top > -INFINITY);
+      if (__any_sync(0xffffffffu, grown || j == 0)) {
+        const float now = grown ? top : mine.m, alpha = grown ? exp2_fast(mine.m - now) : 1.0f;
+        mine.m = now;
+        mine.l *= alpha;
+        if (j > 0) {
+          if (!wait(kBarSums + tile, j - 1))
+            break;
+          tcgen05_fence_after_thread_sync();
+#pragma unroll 1
+          for (int ch = 0; ch < kDim / 32; ++ch) {
+            uint32_t o[16];
+            const uint32_t at = sums + half * (kDim / 2) + ch * 16;
+            tmem_ld_32x32b<16>(at, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x16(at, o);
+          }
+        }
+        weigh(mine.m == -INFINITY ? 0.0f : mine.m);
+      }
+      mine.l += (parts[0].x + parts[0].y) + (parts[1].x + parts[1].y);
+      if (!whole && group_flags != 0x0101010101010101ull) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (4 * half + h)));
+          if (flag & 4u) {  // values held at 1/16
+#pragma unroll
+            for (int i = 8 * h; i < 8 * h + 8; ++i)
+              w[i] = half2_bits(__hmul2(bits_half2(w[i]), __float2half2_rn(16.0f)));
+          }
+          if (flag & 8u) {  // a value that is no number: the rows that see its token are none either
+            const uint32_t bad = poison[slot * kTileGroups + 4 * half + h];
+            for (int i = 0; i < kGroupTokens; ++i)
+              if (((bad >> i) & 1u) && 16 * h + i <= upper && 16 * h + i >= lower)
+                mine.l = NAN;
+          }
+        }
+      }
+      tmem_st_32x32b_x16(scores + half * 32, *reinterpret_cast<const uint32_t(*)[16]>(w));
+      tmem_st_32x32b_x16(scores + half * 32 + 16, *reinterpret_cast<const uint32_t(*)[16]>(w + 16));
+      tmem_st_wait();
+      tcgen05_fence_before_thread_sync();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars[kBarWeights + tile]);
+      if (tiles_q == 2) {
+        const State swap = mine;
+        mine = other;
+        other = swap;
+      }
+    }
+    // ---- the rows' results, each thread half of the elements; element n of the sums is
+    // d = 32 (n / 32) + 16 ((n >> 4) & 1) + 2 (n & 7) + ((n >> 3) & 1)
+    const bool vector = (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0 && ((c.out_row_stride | c.out_head_stride) & 7u) == 0;
+#pragma unroll 1
+    for (int tile = 0; tile < tiles_q; ++tile) {
+      const State &st = tile == 0 ? mine : other;
       bool done = tiles > 0 && *abort_flag == 0;
       if (done) {
         done = wait(kBarSums + tile, tiles - 1);
         tcgen05_fence_after_thread_sync();
       }
-      const bool mine = pair < rows;
-      const size_t q_head = static_cast<size_t>(head) * p.group + (pair - token * static_cast<int32_t>(p.group));
+      // the row's sum is in two threads
+      float *exchange = tops + ((steps + tile + 1) & 1) * 256;
+      exchange[half * 128 + row] = st.l;
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars[kBarPair + (warp & 3)]);
+      float l = st.l;
+      if (wait(kBarPair + (warp & 3), steps + 1 + tile))
+        l = half == 0 ? l + exchange[128 + row] : exchange[row] + l;
+      const int32_t pair = pair0 + tile * kTileRows + row, token = pair / group;
+      const size_t q_head = static_cast<size_t>(head) * group + (pair - token * group);
       const size_t at = static_cast<size_t>(q.first_row + token) * c.out_row_stride + q_head * c.out_head_stride;
-      const bool vector = (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0 && ((c.out_row_stride | c.out_head_stride) & 7u) == 0;
-      const size_t slot = (static_cast<size_t>(blockIdx.x) * 2 + tile) * kTileRows + row0 + lane;
+      const size_t slot = (static_cast<size_t>(blockIdx.x) * 2 + tile) * kTileRows + row;
       float *part_sums = p.splits > 1 ? reinterpret_cast<float *>(static_cast<uint8_t *>(c.workspace) + prefill_sums_offset(gridDim.x)) + slot * kDim : nullptr;
-      const float factor = p.splits > 1 ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
+      const bool any = done && (l > 0.0f || l != l);
+      const float factor = !any ? 0.0f : p.splits > 1 ? 1.0f : 1.0f / l;
+#pragma unroll 1
+      for (int b = half * (NB / 2); b < (half + 1) * (NB / 2); ++b) {
         uint32_t o[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          o[i] = 0;
-        if (done) {
-          tmem_ld_32x32b<32>(sums + b * 32, o);
-          tmem_ld_wait();
-        }
+        tmem_ld_32x32b<32>(tmem + quadrant + 256 + tile * kDim + b * 32, o);
+        tmem_ld_wait();
         float y[32];
 #pragma unroll
         for (int d = 0; d < 32; ++d) {
           const float v = __uint_as_float(o[(d >> 4) * 16 + (d & 1) * 8 + ((d & 15) >> 1)]);
-          y[d] = l > 0.0f || l != l ? v * factor : 0.0f;
+          y[d] = any ? v * factor : 0.0f;  // (without a product the columns hold anything)
         }
-        if (mine) {
+        if (pair < rows) {
           if (part_sums != nullptr) {
 #pragma unroll
             for (int d = 0; d < 32; d += 4)
@@ -468,17 +524,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           } else if (vector) {
 #pragma unroll
             for (int d = 0; d < 32; d += 8) {
-              uint32_t w[4];
+              uint32_t v[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 if (c.type == TCRV_CUDA_TYPE_F16) {
-                  w[i] = half2_bits(__floats2half2_rn(y[d + 2 * i], y[d + 2 * i + 1]));
+                  v[i] = half2_bits(__floats2half2_rn(y[d + 2 * i], y[d + 2 * i + 1]));
                 } else {
                   const __nv_bfloat162 h = __floats2bfloat162_rn(y[d + 2 * i], y[d + 2 * i + 1]);
-                  memcpy(&w[i], &h, 4);
+                  memcpy(&v[i], &h, 4);
                 }
               }
-              *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(c.out) + at + b * 32 + d) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(c.out) + at + b * 32 + d) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           } else {
 #pragma unroll
@@ -487,12 +543,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           }
         }
       }
-      if (mine) {
+      if (pair < rows && half == 0) {
         if (part_sums != nullptr)
-          *reinterpret_cast<float2 *>(static_cast<float *>(c.workspace) + slot * 2) = make_float2(m, l);
+          *reinterpret_cast<float2 *>(static_cast<float *>(c.workspace) + slot * 2) = make_float2(st.m, done ? l : 0.0f);
         else if (c.lse != nullptr)
-          c.lse[static_cast<size_t>(q.first_row + token) * c.heads + q_head] =
-              l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+          c.lse[static_cast<size_t>(q.first_row + token) * c.heads + q_head] = any ? (st.m + log2f(l)) * 0.6931471805599453f : -INFINITY;
       }
     }
   } else if (warp < kProductWarp) {
@@ -541,53 +596,44 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         }
       }
     };
-    RawGroup<NB> now, ahead;
-    ask();
-    fetch(ahead);
-    ask();
-#pragma unroll 1
-    for (int j = 0; j < tiles; ++j) {
+    // this lane's places in the operands; neighbouring lanes' chunks fall on different banks
+    uint8_t *const key_even = smem + L::kKey + (w * kGroupTokens + g) * 128 + (((2 * t) ^ g) << 4);
+    uint8_t *const key_odd = smem + L::kKey + (w * kGroupTokens + g) * 128 + (((2 * t + 1) ^ g) << 4);
+    uint8_t *const value_first = smem + L::kValue + (w >> 2) * (kDim * 128) + g * 128 + t * 4 + ((((w & 3) * 2) ^ g) << 4);
+    uint8_t *const value_second = smem + L::kValue + (w >> 2) * (kDim * 128) + g * 128 + t * 4 + ((((w & 3) * 2 + 1) ^ g) << 4);
+    const auto convert = [&](RawGroup<NB> &now, int j) -> bool {
       const int stage = j & 1, slot = j % kSlots;
-      now = ahead;
-      fetch(ahead);
-      ask();
       // ---- scales: of values, two tokens side by side; none for tokens behind the context; large ones are seen to
-      const int32_t left = q.len - ((tile_begin + j) * kTileGroups + w) * kGroupTokens;
-      uint32_t large_key = 0, large_value = 0;
+      uint32_t pair[2][NB];
+      uint32_t some = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t pair[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          pair[b] = __byte_perm(now.value_scale[h][b / 2], now.value_scale[h][NB / 2 + b / 2], (b & 1) ? 0x7632 : 0x5410);
+        for (int b = 0; b < NB; ++b) {
+          pair[h][b] = __byte_perm(now.value_scale[h][b / 2], now.value_scale[h][NB / 2 + b / 2], (b & 1) ? 0x7632 : 0x5410);
+          some |= now.value_scale[h][b];
+        }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          now.value_scale[h][b] = pair[b];
+        for (int b = 0; b < NB / 2; ++b)
+          some |= now.key_scale[h][b];
       }
+      const int32_t left = q.len - ((tile_begin + j) * kTileGroups + w) * kGroupTokens;
       if (left < kGroupTokens) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t keep = (2 * t + 8 * h < left ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < left ? 0xffff0000u : 0u);
 #pragma unroll
           for (int b = 0; b < NB; ++b)
-            now.value_scale[h][b] &= keep;
+            pair[h][b] &= keep;
 #pragma unroll
           for (int b = 0; b < NB / 2; ++b)
             now.key_scale[h][b] = g + 8 * h < left ? now.key_scale[h][b] : 0;
         }
       }
-      // |d| >= 2^13, with infinities and NaN: 8 d may leave fp16
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int b = 0; b < NB / 2; ++b)
-          large_key |= (now.key_scale[h][b] & 0x7fff7fffu) + 0x10001000u;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          large_value |= (now.value_scale[h][b] & 0x7fff7fffu) + 0x10001000u;
-      }
       uint32_t flag = now.there ? 1u : 0u;
-      if (__any_sync(0xffffffffu, ((large_key | large_value) & 0x80008000u) != 0)) {
+      // a scale of 2^13 or more (8 d may leave fp16), an infinity or a NaN has these three bits; so may several others together,
+      // which does no harm
+      if (__any_sync(0xffffffffu, (some & 0x7000u) == 0x7000u || (some & 0x70000000u) == 0x70000000u)) {
         const __half2 sixteenth = __float2half2_rn(0.0625f);
         uint32_t bad = 0;
 #pragma unroll
@@ -597,15 +643,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
             now.key_scale[h][b] = half2_bits(__hmul2(bits_half2(now.key_scale[h][b]), sixteenth));
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            if ((now.value_scale[h][b] & 0x7c00u) == 0x7c00u) {
+            if ((pair[h][b] & 0x7c00u) == 0x7c00u) {
               bad |= 1u << (2 * t + 8 * h);
-              now.value_scale[h][b] &= 0xffff0000u;
+              pair[h][b] &= 0xffff0000u;
             }
-            if ((now.value_scale[h][b] & 0x7c000000u) == 0x7c000000u) {
+            if ((pair[h][b] & 0x7c000000u) == 0x7c000000u) {
               bad |= 2u << (2 * t + 8 * h);
-              now.value_scale[h][b] &= 0xffffu;
+              pair[h][b] &= 0xffffu;
             }
-            now.value_scale[h][b] = half2_bits(__hmul2(bits_half2(now.value_scale[h][b]), sixteenth));
+            pair[h][b] = half2_bits(__hmul2(bits_half2(pair[h][b]), sixteenth));
           }
         }
         bad = __reduce_or_sync(0xffffffffu, bad);
@@ -614,11 +660,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           poison[slot * kTileGroups + w] = static_cast<uint16_t>(bad);
       }
       if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
-        break;
+        return false;
       if (lane == 0)
         flags[slot * kTileGroups + w] = static_cast<uint8_t>(flag);
-      // ---- keys: a word's 8 elements are 16 bytes of the token's row; neighbouring lanes' chunks fall on different banks
-      uint8_t *keys = smem + L::kKey + stage * L::kKeyBytes + (w * kGroupTokens + g) * 128;
+      // ---- keys: a word's 8 elements are 16 bytes of the token's row
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -629,7 +674,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
                                      half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
                                      half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
                                      half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale)));
-          *reinterpret_cast<uint4 *>(keys + (b >> 1) * L::kPanel + h * 1024 + (((2 * t + (b & 1)) ^ g) << 4)) = v;
+          *reinterpret_cast<uint4 *>(((b & 1) ? key_odd : key_even) + stage * L::kKeyBytes + (b >> 1) * L::kPanel + h * 1024) = v;
         }
       }
       fence_proxy_async();
@@ -638,52 +683,70 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         mbar_arrive(&bars[kBarKeyFull + stage]);
       // ---- values, transposed: row n of the operand is an element, its columns the tokens
       if (j >= 2 && !wait(kBarValueFree + stage, (j >> 1) - 1))
-        break;
-      uint8_t *values = smem + L::kValue + stage * L::kValueBytes + (w >> 2) * (kDim * 128) + g * 128 + t * 4;
+        return false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint8_t *column = values + ((((w & 3) * 2 + h) ^ g) << 4);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint32_t word = now.value[h][b];
-          const __half2 scale = bits_half2(now.value_scale[h][b]);
+          const __half2 scale = bits_half2(pair[h][b]);
           const uint32_t v[4] = {half2_bits(__hmul2(bits_half2(low_nibbles(word)), scale)),
                                  half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
                                  half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
                                  half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale))};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint32_t *>(column + (b * 4 + k) * 1024) = v[k];
+            *reinterpret_cast<uint32_t *>((h ? value_second : value_first) + stage * L::kValueBytes + (b * 4 + k) * 1024) = v[k];
         }
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&bars[kBarValueFull + stage]);
+      return true;
+    };
+    // Two tiles' groups are on their way; each register set is filled again as soon as it has been used, without a copy.
+    RawGroup<NB> even, odd;
+    ask();
+    fetch(even);
+    ask();
+    fetch(odd);
+    ask();
+#pragma unroll 1
+    for (int j = 0; j < tiles; j += 2) {
+      if (!convert(even, j))
+        break;
+      fetch(even);
+      ask();
+      if (j + 1 >= tiles || !convert(odd, j + 1))
+        break;
+      fetch(odd);
+      ask();
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegs));
     if (warp == kProductWarp && tiles > 0) {
     // ================================================================ products: one lane issues
-    const uint32_t base = smem_addr(smem);
+    // (values that the compiler knows to be the same in every lane go to the instruction without a detour)
+    const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0), columns = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint32_t kScoreDesc = umma_idesc_f16(kTileRows, kTileTokens), kSumDesc = umma_idesc_f16(kTileRows, kDim);
     const bool leader = elect_one();
     const auto score = [&](int tile, int stage) {
-      const uint64_t a = umma_desc_k_major_sw128(base + L::kQuery + tile * L::kKeyBytes);
-      const uint64_t b = umma_desc_k_major_sw128(base + L::kKey + stage * L::kKeyBytes);
+      const uint32_t a = desc_low(base + L::kQuery + tile * L::kKeyBytes), b = desc_low(base + L::kKey + stage * L::kKeyBytes);
+      umma_f16_ss<false>(columns + tile * 128, a, b, kScoreDesc);
 #pragma unroll
-      for (int k = 0; k < kDim / 16; ++k) {
+      for (int k = 1; k < kDim / 16; ++k) {
         const uint32_t at = (k / 4) * (L::kPanel >> 4) + (k % 4) * 2;
-        umma_f16_ss(tmem + tile * 128, a + at, b + at, kScoreDesc, k > 0);
+        umma_f16_ss<true>(columns + tile * 128, a + at, b + at, kScoreDesc);
       }
       umma_commit(&bars[kBarScores + tile]);
     };
     const auto sum = [&](int tile, int stage, bool add) {
-      const uint64_t b = umma_desc_k_major_sw128(base + L::kValue + stage * L::kValueBytes);
+      const uint32_t b = desc_low(base + L::kValue + stage * L::kValueBytes);
 #pragma unroll
       for (int k = 0; k < kTileTokens / 16; ++k) {
         const uint32_t at = (k / 4) * ((kDim * 128) >> 4) + (k % 4) * 2;
-        umma_f16_ts(tmem + 256 + tile * kDim, tmem + tile * 128 + k * 8, b + at, kSumDesc, add || k > 0);
+        umma_f16_ts(columns + 256 + tile * kDim, columns + tile * 128 + k * 8, b + at, kSumDesc, k > 0 || add ? 1u : 0u);
       }
       umma_commit(&bars[kBarSums + tile]);
     };
