@@ -77,6 +77,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // 8 x 8 transpose of 16-bit elements held two to a lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -101,14 +109,62 @@ __device__ __forceinline__ __half2 bits_half2(uint32_t u) {
   return h;
 }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t"
+      "}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t"
+      "}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t"
+      "}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Two nibbles n at bits 0..3 and 16..19 -> the fp16 pair n - 8: OR-ed into 1024.0 they are 1024 + n, and
 // the subtraction is exact.  At bits 4..7 and 20..23 they make 1024 + 16 n: times 1/16, less 72.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t u;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w), "r"(mask), "r"(bits));  // one instruction: (w & mask) | bits
+  return u;
+}
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t w) {
-  const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
+  const uint32_t u = and_or(w, 0x000f000fu, 0x64006400u);
   return half2_bits(__hsub2(bits_half2(u), bits_half2(0x64086408u)));
 }
 __device__ __forceinline__ uint32_t high_nibbles(uint32_t w) {
-  const uint32_t u = (w & 0x00f000f0u) | 0x64006400u;
+  const uint32_t u = and_or(w, 0x00f000f0u, 0x64006400u);
   return half2_bits(__hfma2(bits_half2(u), bits_half2(0x2c002c00u), bits_half2(0xd480d480u)));
 }
 
@@ -192,25 +248,24 @@ __device__ __forceinline__ long long request_work(const ColumnParams &p, const R
   return static_cast<long long>(q.units) * q.column_groups * static_cast<long long>(p.call.cache.kv_heads);
 }
 
-// A place in the list of all units: requests, then kv heads, then column groups, then units.
+// A segment (kv head and column group of a request) of the list of all units: requests, then kv heads, then column groups,
+// then units.  Its ends count from the CTA's first unit; one that lies beyond 31 bits is as good as that.
 struct Cursor {
   uint32_t r;
   Request q;
-  long long request_begin;  // first unit of the request
-  int32_t segment;          // head * column_groups + column group
-  __device__ __forceinline__ long long begin() const { return request_begin + static_cast<long long>(segment) * q.units; }
-  __device__ __forceinline__ long long end() const { return begin() + q.units; }
+  int32_t segment;  // head * column_groups + column group
+  int32_t begin, end;
   // moves to the segment that holds unit u, which is not before this one (u is inside the list)
-  __device__ __forceinline__ void seek(const ColumnParams &p, long long u, int group_rows) {
-    while (u >= end()) {
-      const int32_t segments = q.column_groups * static_cast<int32_t>(p.call.cache.kv_heads);
-      if (++segment < segments)
-        continue;
-      request_begin += static_cast<long long>(segments) * q.units;
-      segment = 0;
-      do
-        q = load_request(p, ++r, group_rows);
-      while (q.units == 0);
+  __device__ __forceinline__ void seek(const ColumnParams &p, int32_t u, int group_rows) {
+    while (u >= end) {
+      begin = end;
+      if (++segment == q.column_groups * static_cast<int32_t>(p.call.cache.kv_heads)) {
+        segment = 0;
+        do
+          q = load_request(p, ++r, group_rows);
+        while (q.units == 0);
+      }
+      end = begin + q.units;
     }
   }
 };
@@ -254,8 +309,9 @@ __device__ __forceinline__ long long find_start(const ColumnParams &p, int group
           break;
         before += w;
       }
-      c.request_begin = before;
       c.segment = static_cast<int32_t>((u - before) / c.q.units);
+      c.begin = static_cast<int32_t>(before + static_cast<long long>(c.segment) * c.q.units - u);
+      c.end = c.begin + c.q.units;
       *out = c;
     }
   }
@@ -308,33 +364,36 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       ranges[blockIdx.x].valid = 0;
     return;
   }
-  const long long u0 = cta_begin(work, blockIdx.x, ctas), u1 = cta_begin(work, blockIdx.x + 1, ctas);
+  const long long u0 = cta_begin(work, blockIdx.x, ctas);
+  const int32_t units = static_cast<int32_t>(cta_begin(work, blockIdx.x + 1, ctas) - u0);  // of this CTA, counted from 0
 
-  // ---- this warp's copies: units u0 + warp, u0 + warp + kWarps, ...  Lanes 0 and 1 copy a group each; the
-  // page of the unit to come is read one step before its copy, so that the copy never waits for the table.
+  // ---- this warp's copies: units warp, warp + kWarps, ...  Lanes 0 and 1 copy a group each; the page of the unit to
+  // come is read one step before its copy, so that the copy never waits for the table.
   Cursor ahead = start;
-  long long next = u0 + warp;  // unit whose pages are in `page`
+  int32_t next = warp;  // unit whose pages are asked for
   const uint8_t *source = nullptr;
+  const uint32_t per_page = static_cast<uint32_t>(c.cache.groups);
+  const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
+  int32_t page = -1;
+  size_t place = 0;
   auto fetch_page = [&]() {
-    source = nullptr;
-    if (next >= u1)
+    page = -1;
+    if (next >= units)
       return;
     ahead.seek(p, next, kRows);
     if (lane < kUnitGroups) {
-      const int64_t group = static_cast<int64_t>(ahead.q.first_unit + (next - ahead.begin())) * kUnitGroups + lane;
-      if (group * kGroupTokens < ahead.q.len) {
-        const uint32_t at = static_cast<uint32_t>(group / static_cast<uint32_t>(c.cache.groups));
-        const uint32_t in_page = static_cast<uint32_t>(group) - at * static_cast<uint32_t>(c.cache.groups);
-        const int32_t page = c.block_table[ahead.r * c.table_stride + at];
-        const uint32_t head = ahead.segment / ahead.q.column_groups;
-        if (page >= 0 && static_cast<size_t>(page) < c.cache.pages)
-          source = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
-                   (static_cast<size_t>(head) * c.cache.groups + in_page) * kGroupBytes;
+      const uint32_t group = static_cast<uint32_t>(ahead.q.first_unit + (next - ahead.begin)) * kUnitGroups + lane;
+      if (static_cast<int32_t>(group) * kGroupTokens < ahead.q.len) {
+        const uint32_t at = page_shift >= 0 ? group >> page_shift : group / per_page;
+        const uint32_t head = ahead.q.column_groups == 1 ? ahead.segment : ahead.segment / ahead.q.column_groups;
+        page = c.block_table[ahead.r * c.table_stride + at];
+        place = static_cast<size_t>(head * per_page + (group - at * per_page)) * kGroupBytes;
       }
     }
   };
   auto issue = [&](int stage) {
-    if (next < u1) {
+    if (next < units) {
+      source = page >= 0 && static_cast<size_t>(page) < c.cache.pages ? c.cache.data + static_cast<size_t>(page) * c.cache.page_stride + place : nullptr;
       const uint32_t there = __ballot_sync(0xffffffffu, source != nullptr) & 3u;
       if (lane == 0) {
         flags[stage] = there;
@@ -356,10 +415,10 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
   bool failed = false;
 
   Cursor at = start;
-  long long u = u0 + warp;
-  for (long long from = u0; from < u1;) {
+  int32_t u = warp;
+  for (int32_t from = 0; from < units;) {
     at.seek(p, from, kRows);
-    const long long seg_begin = at.begin(), seg_end = at.end(), to = seg_end < u1 ? seg_end : u1;
+    const int32_t seg_begin = at.begin, seg_end = at.end, to = seg_end < units ? seg_end : units;
     const int32_t head = at.segment / at.q.column_groups, column_group = at.segment - head * at.q.column_groups;
     const int32_t pair0 = column_group * kRows, pairs = min(kRows, at.q.rows * static_cast<int32_t>(p.group) - pair0);
 
@@ -439,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       }
       const uint8_t *unit = ring + stage * L::kUnitBytes;
       const uint32_t there = flags[stage];
-      const int32_t token0 = static_cast<int32_t>(at.q.first_unit + (u - seg_begin)) * kUnitTokens;
+      const int32_t token0 = (at.q.first_unit + (u - seg_begin)) * kUnitTokens;
 
       // ---- S^T = K q^T
       float s[kUnitGroups][NT][4];
@@ -453,24 +512,22 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         load_scales<NB>(d0, group + 512 * NB + g * NB * 2);
         load_scales<NB>(d1, group + 512 * NB + (g + 8) * NB * 2);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[gr][j][e] = 0.0f;
-#pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint32_t a0[4] = {low_nibbles(w0[b]), low_nibbles(w1[b]), low_nibbles(w0[b] >> 8), low_nibbles(w1[b] >> 8)};
           const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w1[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b] >> 8)};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const uint4 q = *reinterpret_cast<const uint4 *>(smem + L::kQuery + ((j * NB + b) * 32 + lane) * 16);
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(acc, a0, q.x, q.y);
+            float acc[4];
+            mma16816_zero(acc, a0, q.x, q.y);
             mma16816(acc, a1, q.z, q.w);
-            s[gr][j][0] = fmaf(acc[0], d0[b], s[gr][j][0]);
-            s[gr][j][1] = fmaf(acc[1], d0[b], s[gr][j][1]);
-            s[gr][j][2] = fmaf(acc[2], d1[b], s[gr][j][2]);
-            s[gr][j][3] = fmaf(acc[3], d1[b], s[gr][j][3]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = make_float2(acc[2 * h], acc[2 * h + 1]), d = h ? make_float2(d1[b], d1[b]) : make_float2(d0[b], d0[b]);
+              const float2 y = b == 0 ? mul2(x, d) : fma2(x, d, make_float2(s[gr][j][2 * h], s[gr][j][2 * h + 1]));
+              s[gr][j][2 * h] = y.x;
+              s[gr][j][2 * h + 1] = y.y;
+            }
           }
         }
       }
@@ -592,8 +649,9 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
             for (int h = 0; h < 2; ++h) {
               float x0, x1;
               if constexpr (TERMS == 1) {
-                x0 = pr[gr][j][h][0] * vd[gr][h][b];
-                x1 = pr[gr][j][h][1] * vd[gr][h][b];
+                const float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][1]), make_float2(vd[gr][h][b], vd[gr][h][b]));
+                x0 = x.x;
+                x1 = x.y;
                 if (!whole) {  // a weight of zero stays zero, whatever the scale
                   x0 = pr[gr][j][h][0] == 0.0f ? 0.0f : x0;
                   x1 = pr[gr][j][h][1] == 0.0f ? 0.0f : x1;
@@ -635,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         }
       }
     __syncthreads();
-    const bool first = seg_begin < u0, split = first || seg_end > u1;
+    const bool first = seg_begin < 0, split = first || seg_end > units;
     const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
     uint8_t *ws = static_cast<uint8_t *>(c.workspace);
     float *part_stats = reinterpret_cast<float *>(ws + column_stats_offset(gridDim.x)) + slot * kRows * 2;
@@ -699,17 +757,18 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       }
       __syncthreads();
     }
-    if (threadIdx.x == 0 && to == u1) {
+    if (threadIdx.x == 0 && to == units) {
       SplitRange range = {};
-      range.valid = !first && seg_end > u1;
+      range.valid = !first && seg_end > units;
       range.request = static_cast<int32_t>(at.r);
       range.head = head;
       range.column_group = column_group;
       if (range.valid) {  // the CTA that holds the segment's last unit
-        int last = static_cast<int>((seg_end - 1) * ctas / work);
-        while (last + 1 < ctas && cta_begin(work, last + 1, ctas) < seg_end)
+        const long long end = u0 + seg_end;
+        int last = static_cast<int>((end - 1) * ctas / work);
+        while (last + 1 < ctas && cta_begin(work, last + 1, ctas) < end)
           ++last;
-        while (cta_begin(work, last, ctas) >= seg_end)
+        while (cta_begin(work, last, ctas) >= end)
           --last;
         range.last_cta = last;
       }
