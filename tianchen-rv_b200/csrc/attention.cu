@@ -16,7 +16,7 @@ constexpr size_t kPrefillRows = 33;
 
 struct Shape {
   // the columns kernel
-  int tiles, terms, rows;  // rows: query rows of a column group
+  int tiles, terms, rows;  // rows: query rows of a column group, 8 to a tile
   int grid;
   long long most_rows;
   // the prefill kernel
@@ -33,14 +33,12 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   s.prefill = all >= kPrefillRows && c.type != TCRV_CUDA_TYPE_F32 && (c.cache.dim == 64 || c.cache.dim == 128);
   const size_t rows = s.prefill ? kPrefillRows - 1 : all;
   s.most_rows = static_cast<long long>(rows);
-  // columns (rows times their f32 terms) that one pass over a context takes, in tiles of 8: the fewest that hold all
-  // rows of a request, up to the tiles whose accumulators fit the registers
-  const int most_tiles = c.cache.dim <= 128 ? 4 : 2;
-  for (s.tiles = 1; s.tiles < most_tiles && rows * s.terms > static_cast<size_t>(8 * s.tiles);)
-    s.tiles *= 2;
-  s.rows = s.tiles * 8 / s.terms;
+  // the rows that one pass over a context takes, in tiles of 8: as many as have room for their sums in registers, dealt out evenly
+  const size_t most_rows = 8 * (c.cache.dim <= 64 ? 4 : c.cache.dim <= 128 ? 3 : c.cache.dim <= 192 ? 2 : 1);
+  const size_t groups = (rows + most_rows - 1) / most_rows;
+  s.tiles = static_cast<int>(((rows + groups - 1) / groups + 7) / 8);
+  s.rows = 8 * s.tiles;
   const size_t units = (c.width * c.cache.groups + kUnitGroups - 1) / kUnitGroups;
-  const size_t groups = (rows + s.rows - 1) / s.rows;
   const double most = static_cast<double>(units ? units : 1) * groups * c.cache.kv_heads * c.requests / kWarps + 1;
   const int cap = sm_count() * ctas_per_sm(static_cast<int>(c.cache.dim / 32), s.tiles);
   s.grid = most < cap ? static_cast<int>(most) : cap;
@@ -99,24 +97,30 @@ int launch_columns(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
   return TCRV_CUDA_OK;
 }
 
-template <int NB>
-int launch_dim(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
-  if (s.terms == 1) {
-    if (s.tiles == 1)
-      return launch_columns<NB, 1, 1>(p, s, stream);
-    if (s.tiles == 2)
-      return launch_columns<NB, 2, 1>(p, s, stream);
-    if constexpr (NB <= 4)
-      return launch_columns<NB, 4, 1>(p, s, stream);
-  } else {
-    if (s.tiles == 1)
-      return launch_columns<NB, 1, 2>(p, s, stream);
-    if (s.tiles == 2)
-      return launch_columns<NB, 2, 2>(p, s, stream);
-    if constexpr (NB <= 4)
-      return launch_columns<NB, 4, 2>(p, s, stream);
+template <int NB, int TERMS>
+int launch_tiles(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
+  switch (s.tiles) {
+    case 1:
+      return launch_columns<NB, 1, TERMS>(p, s, stream);
+    case 2:
+      if constexpr (NB <= 6)
+        return launch_columns<NB, 2, TERMS>(p, s, stream);
+      break;
+    case 3:
+      if constexpr (NB <= 4)
+        return launch_columns<NB, 3, TERMS>(p, s, stream);
+      break;
+    case 4:
+      if constexpr (NB <= 2)
+        return launch_columns<NB, 4, TERMS>(p, s, stream);
+      break;
   }
   return TCRV_CUDA_ERR_UNSUPPORTED;
+}
+
+template <int NB>
+int launch_dim(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
+  return s.terms == 1 ? launch_tiles<NB, 1>(p, s, stream) : launch_tiles<NB, 2>(p, s, stream);
 }
 
 template <int NB>

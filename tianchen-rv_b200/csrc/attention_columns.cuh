@@ -11,7 +11,7 @@
 // multiplies the soft-max weight, one operand per block.  What is rounded is the query row (scaled by a
 // power of two so that its largest element lies in [2^14, 2^15)) and the weight times the value's scale:
 //   fp16 and bf16 calls: both to one fp16 term, 2^-12 relative (a 16-bit query is exact);
-//   f32 calls: both to two fp16 terms, 2^-22 relative, in neighbouring columns of one tile.  The value
+//   f32 calls: both to two fp16 terms, 2^-22 relative, with a product each into the same sums.  The value
 //   scales are lifted by a power of two that follows the largest one seen, like the running maximum.
 // Maximum, sum and accumulators are f32.
 #pragma once
@@ -57,17 +57,19 @@ inline int ctas_per_sm(int nb, int nt) { return nb * nt <= 4 ? 2 : 1; }
 template <int NB, int NT, int TERMS>
 struct ColumnLayout {
   static constexpr int kDim = 32 * NB;
-  static constexpr int kStages = NB * NT <= 2 ? 4 : NB * NT <= 3 ? 3 : NB >= 6 ? 2 : NB * NT > 4 ? 4 : 2;
+  static constexpr int kStages = NB * NT <= 2 ? 4 : NB * NT <= 3 ? 3 : NB >= 6 ? 2 : NB * NT > 4 ? 4 : 2;  // (what shared memory has room for)
   static constexpr int kUnitBytes = kUnitGroups * 18 * kDim;
-  static constexpr int kTileRows = 8 / TERMS;    // query rows of a tile
+  static constexpr int kTileRows = 8;            // query rows of a tile
   static constexpr int kRows = NT * kTileRows;   // of a column group
   static constexpr int kSums = kStages * kWarps * kUnitBytes;                     // f32 [warp][row of a tile][d]
   static constexpr int kQuery = kSums + kWarps * kTileRows * kDim * 4;            // fp16 operand of the rows
-  static constexpr int kStats = kQuery + NT * NB * 512;                           // f32 [warp][row][max, sum]
+  static constexpr int kQueryBytes = NT * NB * 512;                               // of a term
+  static constexpr int kStats = kQuery + TERMS * kQueryBytes;                     // f32 [warp][row][max, sum]
   static constexpr int kRowInfo = kStats + kWarps * kRows * 2 * 4;                // f32 scale, int position
   static constexpr int kFlags = kRowInfo + kRows * 8;                             // u32 [stage][warp]
   static constexpr int kBars = (kFlags + kStages * kWarps * 4 + 7) / 8 * 8;
   static constexpr int kBytes = kBars + kStages * kWarps * 8;
+  static_assert(kBytes + 512 <= (NB * NT <= 4 ? 113 : 226) * 1024, "shared memory of an SM");
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -189,21 +191,21 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t *p) {
       w[i] = reinterpret_cast<const uint32_t *>(p)[i];
   }
 }
+// A token's NB scales, two to a word.
 template <int NB>
-__device__ __forceinline__ void load_scales(float (&d)[NB], const uint8_t *p) {
+__device__ __forceinline__ void load_scales(uint32_t (&w)[(NB + 1) / 2], const uint8_t *p) {
   if constexpr (NB % 2 == 0) {
-    uint32_t w[NB / 2];
     load_words<NB / 2>(w, p);
-#pragma unroll
-    for (int i = 0; i < NB / 2; ++i) {
-      const float2 f = __half22float2(bits_half2(w[i]));
-      d[2 * i] = f.x, d[2 * i + 1] = f.y;
-    }
   } else {
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-      d[i] = __half2float(reinterpret_cast<const __half *>(p)[i]);
+    for (int i = 0; i < NB; i += 2)
+      w[i / 2] = reinterpret_cast<const uint16_t *>(p)[i] | (i + 1 < NB ? static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i + 1]) << 16 : 0u);
   }
+}
+template <int N>
+__device__ __forceinline__ float scale_of(const uint32_t (&w)[N], int b) {
+  const __half2 h = bits_half2(w[b / 2]);
+  return (b & 1) ? __high2float(h) : __low2float(h);
 }
 
 // What a call asks of one request.
@@ -337,7 +339,7 @@ template <int NB, int NT, int TERMS>
 __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(const __grid_constant__ ColumnParams p) {
   using L = ColumnLayout<NB, NT, TERMS>;
   constexpr int kDim = L::kDim, kStages = L::kStages, kGroupBytes = 18 * kDim, kRows = L::kRows, kTileRows = L::kTileRows;
-  constexpr int kMine = 2 / TERMS;  // query rows of a tile that a lane's two columns belong to
+  constexpr int kMine = 2;  // query rows of a tile that a lane has
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long scratch[kWarps];
   __shared__ Cursor start;
@@ -414,6 +416,58 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
   uint32_t parity = 0;
   bool failed = false;
 
+  // The rows' operand: row i by warp i % kWarps.  The rows of the segment to come are read before the warps' parts of the
+  // present one are joined, and placed meanwhile.
+  float row_values[NT][NB];
+  const auto load_rows = [&](const Cursor &of) {
+    const int32_t head = of.segment / of.q.column_groups, pair0 = (of.segment - head * of.q.column_groups) * kRows;
+    const int32_t pairs = min(kRows, of.q.rows * static_cast<int32_t>(p.group) - pair0);
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const int i = k * kWarps + warp;
+      const int32_t pair = pair0 + i, token = pair / static_cast<int32_t>(p.group);
+      const int32_t q_head = head * static_cast<int32_t>(p.group) + (pair - token * static_cast<int32_t>(p.group));
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        row_values[k][b] = i < pairs ? load_typed(c.q, static_cast<size_t>(of.q.first_row + token) * c.q_row_stride +
+                                                           static_cast<size_t>(q_head) * c.q_head_stride + b * 32 + lane, c.type)
+                                     : 0.0f;
+    }
+  };
+  const auto place_rows = [&](const Cursor &of) {
+    const int32_t pair0 = (of.segment - of.segment / of.q.column_groups * of.q.column_groups) * kRows;
+    const int32_t pairs = min(kRows, of.q.rows * static_cast<int32_t>(p.group) - pair0);
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const int i = k * kWarps + warp;
+      float top = 0.0f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        top = fmaxf(top, fabsf(row_values[k][b]));
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      // 2^power lifts the largest element into [2^14, 2^15); a row of zeros, or one with an infinity, stays
+      const int power = top > 0.0f && top < INFINITY ? min(120, 141 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
+      const float lift = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+      const int kstep = lane >> 4, f = lane & 15;
+      __half *operand = reinterpret_cast<__half *>(smem + L::kQuery);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const float v = row_values[k][b] * lift;
+        const __half hi = __float2half_rn(v);
+        const int place = (((k * NB + b) * 32 + warp * 4 + (f >> 2)) * 4 + kstep * 2 + (f & 1)) * 2 + ((f & 2) >> 1);
+        operand[place] = hi;
+        if constexpr (TERMS == 2)
+          operand[place + L::kQueryBytes / 2] = isfinite(v) ? __float2half_rn(v - __half2float(hi)) : __float2half_rn(0.0f);
+      }
+      if (lane == 0) {
+        row_scale[i] = c.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+        row_position[i] = i < pairs ? of.q.len - of.q.rows + (pair0 + i) / static_cast<int32_t>(p.group) : -1;
+      }
+    }
+  };
+
   Cursor at = start;
   int32_t u = warp;
   for (int32_t from = 0; from < units;) {
@@ -422,45 +476,9 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     const int32_t head = at.segment / at.q.column_groups, column_group = at.segment - head * at.q.column_groups;
     const int32_t pair0 = column_group * kRows, pairs = min(kRows, at.q.rows * static_cast<int32_t>(p.group) - pair0);
 
-    // ---- the rows' operand: row `i` by warp i % kWarps
-    for (int i = warp; i < kRows; i += kWarps) {
-      float x[NB];
-      float top = 0.0f;
-      const int32_t pair = pair0 + i, token = pair / static_cast<int32_t>(p.group);
-      const int32_t q_head = head * static_cast<int32_t>(p.group) + (pair - token * static_cast<int32_t>(p.group));
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        x[b] = 0.0f;
-        if (i < pairs)
-          x[b] = load_typed(c.q, static_cast<size_t>(at.q.first_row + token) * c.q_row_stride +
-                                     static_cast<size_t>(q_head) * c.q_head_stride + b * 32 + lane, c.type);
-        top = fmaxf(top, fabsf(x[b]));
-      }
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      // 2^k lifts the largest element into [2^14, 2^15); a row of zeros, or one with an infinity, stays
-      int k = 0;
-      if (top > 0.0f && top < INFINITY)
-        k = min(120, 14 - ilogbf(top));
-      const float lift = exp2f(static_cast<float>(k));
-      const int e = lane & 31, kstep = e >> 4, f = e & 15;
-      const int tile = i / kTileRows, n = (i - tile * kTileRows) * TERMS;
-      __half *operand = reinterpret_cast<__half *>(smem + L::kQuery);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const float v = x[b] * lift;
-        const __half hi = __float2half_rn(v);
-        const int place = (((tile * NB + b) * 32 + n * 4 + (f >> 2)) * 4 + kstep * 2 + (f & 1)) * 2 + ((f & 2) >> 1);
-        operand[place] = hi;
-        if constexpr (TERMS == 2)  // the column after it: lanes 4 further on
-          operand[place + 4 * 8] = isfinite(v) ? __float2half_rn(v - __half2float(hi)) : __float2half_rn(0.0f);
-      }
-      if (lane == 0) {
-        row_scale[i] = c.scale * kLog2e * exp2f(static_cast<float>(-k));
-        row_position[i] = i < pairs ? at.q.len - at.q.rows + token : -1;
-      }
-    }
+    if (from == 0)
+      load_rows(at);
+    place_rows(at);  // (no warp is still in the products of the segment before)
     __syncthreads();
     float scale[NT][kMine];
     int32_t position[NT][kMine];
@@ -468,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
+        const int row = j * kTileRows + 2 * t + i;
         scale[j][i] = row_scale[row];
         position[j][i] = row_position[row];
       }
@@ -506,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       for (int gr = 0; gr < kUnitGroups; ++gr) {
         const uint8_t *group = unit + gr * kGroupBytes;
         uint32_t w0[NB], w1[NB];
-        float d0[NB], d1[NB];
+        uint32_t d0[(NB + 1) / 2], d1[(NB + 1) / 2];
         load_words<NB>(w0, group + lane * NB * 4);
         load_words<NB>(w1, group + 128 * NB + lane * NB * 4);
         load_scales<NB>(d0, group + 512 * NB + g * NB * 2);
@@ -515,15 +533,21 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         for (int b = 0; b < NB; ++b) {
           const uint32_t a0[4] = {low_nibbles(w0[b]), low_nibbles(w1[b]), low_nibbles(w0[b] >> 8), low_nibbles(w1[b] >> 8)};
           const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w1[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b] >> 8)};
+          const float e[2] = {scale_of(d0, b), scale_of(d1, b)};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const uint4 q = *reinterpret_cast<const uint4 *>(smem + L::kQuery + ((j * NB + b) * 32 + lane) * 16);
             float acc[4];
             mma16816_zero(acc, a0, q.x, q.y);
             mma16816(acc, a1, q.z, q.w);
+            if constexpr (TERMS == 2) {
+              const uint4 low = *reinterpret_cast<const uint4 *>(smem + L::kQuery + L::kQueryBytes + ((j * NB + b) * 32 + lane) * 16);
+              mma16816(acc, a0, low.x, low.y);
+              mma16816(acc, a1, low.z, low.w);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float2 x = make_float2(acc[2 * h], acc[2 * h + 1]), d = h ? make_float2(d1[b], d1[b]) : make_float2(d0[b], d0[b]);
+              const float2 x = make_float2(acc[2 * h], acc[2 * h + 1]), d = make_float2(e[h], e[h]);
               const float2 y = b == 0 ? mul2(x, d) : fma2(x, d, make_float2(s[gr][j][2 * h], s[gr][j][2 * h + 1]));
               s[gr][j][2 * h] = y.x;
               s[gr][j][2 * h + 1] = y.y;
@@ -546,8 +570,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           for (int gr = 0; gr < kUnitGroups; ++gr)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float v = TERMS == 1 ? s[gr][j][2 * h + i] : s[gr][j][2 * h] + s[gr][j][2 * h + 1];
-              v *= scale[j][i];
+              float v = s[gr][j][2 * h + i] * scale[j][i];
               if (!whole) {
                 const int32_t token = token0 + gr * kGroupTokens + h * 8 + g;
                 if (!((there >> gr) & 1u) || token > position[j][i] || (window && token <= position[j][i] - window))
@@ -575,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         }
 
       // ---- value scales of this lane's tokens; those of unseen tokens may be anything and count as zero
-      float vd[kUnitGroups][2][NB];
+      uint32_t vd[kUnitGroups][2][(NB + 1) / 2];
 #pragma unroll
       for (int gr = 0; gr < kUnitGroups; ++gr)
 #pragma unroll
@@ -584,23 +607,26 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           if (!whole) {
             const bool there_is = ((there >> gr) & 1u) && token0 + gr * kGroupTokens + h * 8 + g < at.q.len;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              vd[gr][h][b] = there_is ? vd[gr][h][b] : 0.0f;
+            for (int b = 0; b < (NB + 1) / 2; ++b)
+              vd[gr][h][b] = there_is ? vd[gr][h][b] : 0u;
           }
         }
       float lift = 1.0f, relift = 1.0f;
       if constexpr (TERMS == 2) {
         const auto largest = [&](bool finite_only) {
-          float top = 0.0f;
+          __half2 most = __float2half2_rn(0.0f);
 #pragma unroll
           for (int gr = 0; gr < kUnitGroups; ++gr)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int b = 0; b < NB; ++b) {
-                const float d = fabsf(vd[gr][h][b]);
-                top = fmaxf(top, finite_only && d == INFINITY ? 0.0f : d);
+              for (int b = 0; b < (NB + 1) / 2; ++b) {
+                uint32_t d = vd[gr][h][b] & 0x7fff7fffu;
+                if (finite_only)
+                  d &= ((d & 0x7c00u) == 0x7c00u ? 0xffff0000u : ~0u) & ((d & 0x7c000000u) == 0x7c000000u ? 0xffffu : ~0u);
+                most = __hmax2(most, bits_half2(d));
               }
+          float top = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
           for (int off = 4; off <= 16; off <<= 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -623,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const float f0 = alpha[j][0] * relift, f1 = alpha[j][kMine - 1] * relift;
+            const float f0 = alpha[j][0] * relift, f1 = alpha[j][1] * relift;
             o[i][j][0] *= f0;
             o[i][j][1] *= f1;
             o[i][j][2] *= f0;
@@ -644,29 +670,27 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b]), high_nibbles(w1[b] >> 8)};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            uint32_t bits[2];
+            uint32_t bits[TERMS][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float x0, x1;
-              if constexpr (TERMS == 1) {
-                const float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][1]), make_float2(vd[gr][h][b], vd[gr][h][b]));
-                x0 = x.x;
-                x1 = x.y;
-                if (!whole) {  // a weight of zero stays zero, whatever the scale
-                  x0 = pr[gr][j][h][0] == 0.0f ? 0.0f : x0;
-                  x1 = pr[gr][j][h][1] == 0.0f ? 0.0f : x1;
-                }
-              } else {
-                float v = pr[gr][j][h][0] * (vd[gr][h][b] * lift);
-                if (!whole)
-                  v = pr[gr][j][h][0] == 0.0f ? 0.0f : v;
-                x0 = __half2float(__float2half_rn(v));
-                x1 = v - x0;
+              const float d = TERMS == 2 ? scale_of(vd[gr][h], b) * lift : scale_of(vd[gr][h], b);
+              float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][1]), make_float2(d, d));
+              if (!whole) {  // a weight of zero stays zero, whatever the scale
+                x.x = pr[gr][j][h][0] == 0.0f ? 0.0f : x.x;
+                x.y = pr[gr][j][h][1] == 0.0f ? 0.0f : x.y;
               }
-              bits[h] = transpose8x8(half2_bits(__floats2half2_rn(x0, x1)));
+              const __half2 hi = __floats2half2_rn(x.x, x.y);
+              bits[0][h] = transpose8x8(half2_bits(hi));
+              if constexpr (TERMS == 2) {
+                const float2 y = __half22float2(hi);
+                bits[1][h] = transpose8x8(half2_bits(__floats2half2_rn(x.x - y.x, x.y - y.y)));
+              }
             }
-            mma16816(o[2 * b][j], a0, bits[0], bits[1]);
-            mma16816(o[2 * b + 1][j], a1, bits[0], bits[1]);
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+              mma16816(o[2 * b][j], a0, bits[term][0], bits[term][1]);
+              mma16816(o[2 * b + 1][j], a1, bits[term][0], bits[term][1]);
+            }
           }
         }
       }
@@ -679,6 +703,11 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     }
 
     // ---- the warps' parts of the segment become one
+    Cursor after = at;
+    if (to < units) {
+      after.seek(p, to, kRows);
+      load_rows(after);
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -686,11 +715,8 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1)
           l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], off);
-        if (g == 0) {
-          const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
-          stats[(warp * kRows + row) * 2] = m[j][i];
-          stats[(warp * kRows + row) * 2 + 1] = l[j][i];
-        }
+        if (g == 0)
+          stats[(warp * kRows + j * kTileRows + 2 * t + i) * 2] = m[j][i];
       }
     __syncthreads();
     const bool first = seg_begin < 0, split = first || seg_end > units;
@@ -700,16 +726,18 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     float *part_sums = reinterpret_cast<float *>(ws + column_sums_offset(gridDim.x, kRows)) + slot * kRows * kDim;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      // this warp's accumulators on the CTA's maximum
+      // this warp's sums on the CTA's maximum
       float f[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int row = j * kTileRows + (TERMS == 1 ? 2 * t + i : t);
+        const int row = j * kTileRows + 2 * t + i;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
           top = fmaxf(top, stats[(w * kRows + row) * 2]);
         f[i] = m[j][i] == -INFINITY ? 0.0f : exp2_fast(m[j][i] - top);
+        if (g == 0)
+          stats[(warp * kRows + row) * 2 + 1] = l[j][i] * f[i];
         if constexpr (TERMS == 2)
           f[i] *= lifted > -100 ? exp2f(static_cast<float>(lifted - 14)) : 1.0f;
       }
@@ -717,45 +745,40 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) {
         const int d = (i >> 1) * 32 + (i & 1) * 16 + 2 * g;
-        if constexpr (TERMS == 1) {
-          *reinterpret_cast<float2 *>(mine + 2 * t * kDim + d) = make_float2(o[i][j][0] * f[0], o[i][j][2] * f[0]);
-          *reinterpret_cast<float2 *>(mine + (2 * t + 1) * kDim + d) = make_float2(o[i][j][1] * f[1], o[i][j][3] * f[1]);
-        } else {
-          *reinterpret_cast<float2 *>(mine + t * kDim + d) =
-              make_float2((o[i][j][0] + o[i][j][1]) * f[0], (o[i][j][2] + o[i][j][3]) * f[0]);
-        }
+        *reinterpret_cast<float2 *>(mine + 2 * t * kDim + d) = make_float2(o[i][j][0] * f[0], o[i][j][2] * f[0]);
+        *reinterpret_cast<float2 *>(mine + (2 * t + 1) * kDim + d) = make_float2(o[i][j][1] * f[1], o[i][j][3] * f[1]);
       }
       __syncthreads();
       for (int i = threadIdx.x; i < kTileRows * kDim; i += kThreads) {
         const int row = j * kTileRows + i / kDim, d = i % kDim;
         if (row >= pairs)
           break;
-        float sum = 0.0f;
+        float sum = 0.0f, total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w)
+        for (int w = 0; w < kWarps; ++w) {
           sum += sums[w * kTileRows * kDim + i];
-        if (split)
-          part_sums[row * kDim + d] = sum;
-        if (!split || d == 0) {
-          float top = -INFINITY, total = 0.0f;
+          total += stats[(w * kRows + row) * 2 + 1];
+        }
+        float top = 0.0f;
+        if (d == 0) {
+          top = -INFINITY;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w)
             top = fmaxf(top, stats[(w * kRows + row) * 2]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float mw = stats[(w * kRows + row) * 2];
-            total += mw == -INFINITY ? 0.0f : exp2_fast(mw - top) * stats[(w * kRows + row) * 2 + 1];
-          }
-          if (split) {
+        }
+        if (split) {
+          part_sums[row * kDim + d] = sum;
+          if (d == 0) {
             part_stats[row * 2] = top;
             part_stats[row * 2 + 1] = total;
-          } else {
-            const int32_t pair = pair0 + row, token = pair / static_cast<int32_t>(p.group);
-            write_row(c, at.q.first_row + token, head * p.group + (pair - token * p.group), d, sum, total, top);
           }
+        } else {
+          const int32_t pair = pair0 + row, token = pair / static_cast<int32_t>(p.group);
+          write_row(c, at.q.first_row + token, head * p.group + (pair - token * p.group), d, sum, total, top);
         }
       }
-      __syncthreads();
+      if (j + 1 < NT)
+        __syncthreads();
     }
     if (threadIdx.x == 0 && to == units) {
       SplitRange range = {};
@@ -774,6 +797,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       }
       ranges[blockIdx.x] = range;
     }
+    at = after;
     from = to;
   }
 }
