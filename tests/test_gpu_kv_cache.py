@@ -49,6 +49,7 @@ def test_store_is_the_row_quantiser_in_the_slots(cuda, pkg, O, kind, dim, heads,
         if n == 41:  # ties of magnitude (the first one decides the sign), zeros, extremes
             k32[5, 0, :32] = np.resize([0.5, -0.5], 32)
             v32[5, 0, :32] = 0
+            v32[7, 0, :32] = -0.0
             k32[6, 0, :32] = 1e-30 if kind != "float16" else 1e-7
             v32[6, 0, :32] = np.resize([3e4, -6e4, 1.0], 32)
             k, v = cuda.from_numpy(k32).to(k.dtype).cuda(), cuda.from_numpy(v32).to(k.dtype).cuda()

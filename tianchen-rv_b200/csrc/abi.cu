@@ -713,7 +713,7 @@ int tcrv_cuda_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_s
     return TCRV_CUDA_OK;
   if (!k || !v || !slots)
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
-  if (rows > kManyRows)
+  if (rows > kManyRows / (cache->kv_heads * cache->dim / TCRV_QK))
     return TCRV_CUDA_ERR_UNSUPPORTED;
   return launch_kv_store_q4_0(type, rows, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, slots, *cache,
                               as_stream(stream));
@@ -730,7 +730,7 @@ int tcrv_cuda_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_
     return TCRV_CUDA_OK;
   if (!k || !v || !slots || reinterpret_cast<uintptr_t>(k) % 16 != 0 || reinterpret_cast<uintptr_t>(v) % 16 != 0)
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
-  if (rows > kManyRows)
+  if (rows > kManyRows / (cache->kv_heads * cache->dim / TCRV_QK))
     return TCRV_CUDA_ERR_UNSUPPORTED;
   return launch_kv_load_q4_0(type, rows, k, v, slots, *cache, as_stream(stream));
 }

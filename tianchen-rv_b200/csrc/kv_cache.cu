@@ -12,10 +12,10 @@ namespace {
 // ------------------------------------------------------------------ store and load
 
 constexpr int kRowThreads = 256;
-constexpr int kTeam = 8;  // lanes to a block of 32 elements: four elements each
+constexpr int kTeam = 4;  // lanes to a block of 32 elements: lane t has elements 4t..4t+3 and 16+4t..16+4t+3, so bytes 4t..4t+3
 
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool vector, float (&v)[4]) {
+__device__ __forceinline__ void load4(const T *p, bool vector, float *v) {
   if (vector) {
     if constexpr (sizeof(T) == 4) {
       const float4 x = *reinterpret_cast<const float4 *>(p);
@@ -35,43 +35,50 @@ __device__ __forceinline__ void load4(const T *p, bool vector, float (&v)[4]) {
   }
 }
 
-// Scale and the nibbles of this lane's four elements, by the rule of quantize_row_q4_0: the scale is
-// the first element of largest magnitude over -8, a quant is trunc(x / d + 8.5), at most 15.  Every
-// step is one IEEE operation, so the blocks are those of the row quantiser, byte for byte.
-__device__ __forceinline__ uint32_t quantise_team(const float (&v)[4], int sub, float *scale) {
-  float best_a = 0.0f, best_v = 0.0f;
-  int best_i = 0x7fffffff;
+// Scale of a block and this lane's four bytes, by the rule of quantize_row_q4_0: the scale is the first element of largest
+// magnitude over -8, a quant is trunc(x / d + 8.5), at most 15.  Every step is one IEEE operation or one that gives its bits
+// (the product with -1/8, a power of two; the reciprocal), so the blocks are those of the row quantiser, byte for byte.
+__device__ __forceinline__ uint32_t quantise_team(const float (&v)[8], float *scale) {
+  float most = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float a = fabsf(v[j]);
-    if (a > best_a) {
-      best_a = a;
-      best_v = v[j];
-      best_i = 4 * sub + j;
-    }
+  for (int j = 0; j < 8; ++j)
+    most = fmaxf(most, fabsf(v[j]));  // (NaN counts as nothing)
+#pragma unroll
+  for (int off = 1; off < kTeam; off <<= 1)
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  // the first element of that magnitude: elements 0..15 lie across the lanes before 16..31 do
+  float low = 0.0f, high = 0.0f;
+  bool in_low = false, in_high = false;
+#pragma unroll
+  for (int j = 3; j >= 0; --j) {
+    const bool l = fabsf(v[j]) == most, h = fabsf(v[4 + j]) == most;
+    low = l ? v[j] : low;
+    high = h ? v[4 + j] : high;
+    in_low |= l;
+    in_high |= h;
   }
+  const int team = threadIdx.x & 28;
+  const uint32_t holders_low = __ballot_sync(0xffffffffu, in_low) >> team & 15u, holders_high = __ballot_sync(0xffffffffu, in_high) >> team & 15u;
+  const float chosen = __shfl_sync(0xffffffffu, holders_low ? low : high, __ffs(holders_low ? holders_low : holders_high) - 1, kTeam);
+  const float best = most > 0.0f ? chosen : 0.0f;
+  const float d = __fmul_rn(best, -0.125f);
+  const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+  uint32_t bytes = 0;
 #pragma unroll
-  for (int off = 1; off < kTeam; off <<= 1) {
-    const float oa = __shfl_xor_sync(0xffffffffu, best_a, off);
-    const float ov = __shfl_xor_sync(0xffffffffu, best_v, off);
-    const int oi = __shfl_xor_sync(0xffffffffu, best_i, off);
-    if (oa > best_a || (oa == best_a && oi < best_i)) {
-      best_a = oa;
-      best_v = ov;
-      best_i = oi;
-    }
-  }
-  const float d = __fdiv_rn(best_v, -8.0f);
-  const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-  uint32_t mine = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int q = static_cast<int>(__fadd_rn(__fmul_rn(v[j], id), 8.5f));
-    mine |= static_cast<uint32_t>(max(0, min(15, q))) << (8 * j);
+  for (int j = 0; j < 8; ++j) {
+    const int q = static_cast<int>(__fadd_rn(__fmul_rn(v[j], id), 8.5f));  // (at least 0: |x / d| <= 8, and 0 for NaN)
+    bytes |= static_cast<uint32_t>(min(15, q)) << (8 * (j & 3) + (j & 4));
   }
   *scale = d;
-  // byte j of a block packs element j with element j + 16: lanes 0..3 hold the low ones
-  return mine | (__shfl_down_sync(0xffffffffu, mine, 4, kTeam) << 4);
+  return bytes;
+}
+
+// log2 of a power of two, -1 for other numbers
+inline int shift_of(uint32_t n) {
+  int s = 0;
+  while (s < 31 && (1u << s) < n)
+    ++s;
+  return (1u << s) == n ? s : -1;
 }
 
 struct RowTensor {
@@ -79,58 +86,59 @@ struct RowTensor {
   size_t row_stride, head_stride;
 };
 
-// One team of eight lanes per (row, head, block), the key's block and the value's; teams run over
-// blocks, then heads, then rows, so a warp reads 4 adjacent blocks.  Bound by bytes: the reads are
-// whole rows; a key's words of one token are adjacent, a value's halfwords lie 4 bytes apart in 8
-// runs of 4 nb (they meet those of the group's other tokens in L2).
-template <typename T, bool kVector>
+// One team of four lanes per (row, head, block), the key's block and the value's; teams run over blocks, then heads, then
+// rows, so a warp reads 8 adjacent blocks.  Bound by instructions, about 20 an element (8191 rows of 8 heads of 128, bf16:
+// 35 us with eight lanes to a block, which pay the item's arithmetic and the shuffles twice); a key's words of one token are
+// adjacent, a value's halfwords lie 4 bytes apart in 8 runs of 4 nb (they meet those of the group's other tokens in L2).
+// kBlocks: blocks to a row, 0 where only the call knows.
+template <typename T, bool kVector, int kBlocks>
 __global__ void __launch_bounds__(kRowThreads)
     kv_store_kernel(RowTensor k, RowTensor v, const int64_t *slots, uint8_t *cache, size_t page_stride, int64_t capacity,
-                    uint32_t page_tokens, uint32_t heads, uint32_t nb, uint32_t rows) {
+                    uint32_t page_tokens, int page_shift, Divisor by_row, Divisor by_block, uint32_t rows) {
   pdl_enter();
-  const int sub = threadIdx.x & (kTeam - 1);
-  const uint32_t per_row = heads * nb;
-  const uint64_t items = static_cast<uint64_t>(rows) * per_row;
+  const int t = threadIdx.x & (kTeam - 1);
+  const uint32_t per_row = by_row.d, nb = kBlocks ? kBlocks : by_block.d;
+  const uint64_t items = static_cast<uint64_t>(rows) * per_row;  // (fewer than 2^32)
   const uint64_t teams = static_cast<uint64_t>(gridDim.x) * (kRowThreads / kTeam);
   // (all teams of a warp make the same number of rounds: the shuffles need every lane)
-  for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kRowThreads / kTeam) + ((threadIdx.x >> 5) << 2); first < items;
-       first += teams) {
-    const uint64_t item = first + ((threadIdx.x & 31) >> 3);
+  for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kRowThreads / kTeam) + ((threadIdx.x >> 5) << 3); first < items; first += teams) {
+    const uint64_t item = first + ((threadIdx.x & 31) / kTeam);
     const bool inside = item < items;
-    const uint32_t row = inside ? static_cast<uint32_t>(item / per_row) : 0;
-    const uint32_t rest = inside ? static_cast<uint32_t>(item - static_cast<uint64_t>(row) * per_row) : 0;
-    const uint32_t head = rest / nb, b = rest - head * nb;
+    const uint32_t row = inside ? by_row.of(static_cast<uint32_t>(item)) : 0;
+    const uint32_t rest = inside ? static_cast<uint32_t>(item) - row * per_row : 0;
+    const uint32_t head = kBlocks ? rest / nb : by_block.of(rest), b = rest - head * nb;
     const int64_t slot = inside ? slots[row] : -1;
     const bool live = slot >= 0 && slot < capacity;
-    float kx[4] = {0.f, 0.f, 0.f, 0.f}, vx[4] = {0.f, 0.f, 0.f, 0.f};
+    float kx[8], vx[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      kx[e] = vx[e] = 0.0f;
     if (live) {
-      const size_t d = b * 32 + 4 * sub;
-      load4(static_cast<const T *>(k.p) + row * k.row_stride + head * k.head_stride + d, kVector, kx);
-      load4(static_cast<const T *>(v.p) + row * v.row_stride + head * v.head_stride + d, kVector, vx);
+      const T *kp = static_cast<const T *>(k.p) + row * k.row_stride + head * k.head_stride + b * 32 + 4 * t;
+      const T *vp = static_cast<const T *>(v.p) + row * v.row_stride + head * v.head_stride + b * 32 + 4 * t;
+      load4(kp, kVector, kx);
+      load4(kp + 16, kVector, kx + 4);
+      load4(vp, kVector, vx);
+      load4(vp + 16, kVector, vx + 4);
     }
     float kd, vd;
-    const uint32_t kq = quantise_team(kx, sub, &kd);
-    const uint32_t vq = quantise_team(vx, sub, &vd);
+    const uint32_t kq = quantise_team(kx, &kd), vq = quantise_team(vx, &vd);
     if (live) {
-      const uint64_t page = static_cast<uint64_t>(slot) / page_tokens;
+      const uint64_t page = page_shift >= 0 ? slot >> page_shift : static_cast<uint64_t>(slot) / page_tokens;
       const uint32_t in_page = static_cast<uint32_t>(slot - page * page_tokens), token = in_page % kGroupTokens;
       uint8_t *group = cache + page * page_stride +
                        static_cast<size_t>(head * (page_tokens / kGroupTokens) + in_page / kGroupTokens) * kv_group_bytes(32 * nb);
-      if (sub < 4) {
-        *reinterpret_cast<uint32_t *>(group + kv_key_word(nb, token, sub, b)) = kq;
-        *reinterpret_cast<uint16_t *>(group + kv_value_half(nb, token, 2 * sub, b)) = static_cast<uint16_t>(vq);
-        *reinterpret_cast<uint16_t *>(group + kv_value_half(nb, token, 2 * sub + 1, b)) = static_cast<uint16_t>(vq >> 16);
-      } else if (sub == 4) {
-        *reinterpret_cast<__half *>(group + kv_key_scale(nb, token, b)) = __float2half_rn(kd);
-      } else if (sub == 5) {
-        *reinterpret_cast<__half *>(group + kv_value_scale(nb, token, b)) = __float2half_rn(vd);
-      }
+      *reinterpret_cast<uint32_t *>(group + kv_key_word(nb, token, t, b)) = kq;
+      *reinterpret_cast<uint16_t *>(group + kv_value_half(nb, token, 2 * t, b)) = static_cast<uint16_t>(vq);
+      *reinterpret_cast<uint16_t *>(group + kv_value_half(nb, token, 2 * t + 1, b)) = static_cast<uint16_t>(vq >> 16);
+      if (t < 2)
+        *reinterpret_cast<__half *>(group + (t == 0 ? kv_key_scale(nb, token, b) : kv_value_scale(nb, token, b))) = __float2half_rn(t == 0 ? kd : vd);
     }
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
+__device__ __forceinline__ void store4(T *p, const float *v) {
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
@@ -144,41 +152,46 @@ __device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
   }
 }
 
-// The same items; lane `sub` gives elements 4 sub .. 4 sub + 3 of its block.
-template <typename T>
+// The same items and lanes.  Bound by the bytes it writes.
+template <typename T, int kBlocks>
 __global__ void __launch_bounds__(kRowThreads)
     kv_load_kernel(T *k, T *v, const int64_t *slots, const uint8_t *cache, size_t page_stride, int64_t capacity,
-                   uint32_t page_tokens, uint32_t heads, uint32_t nb, uint32_t rows) {
+                   uint32_t page_tokens, int page_shift, Divisor by_row, Divisor by_block, uint32_t rows) {
   pdl_enter();
-  const int sub = threadIdx.x & (kTeam - 1), t = sub & 3, shift = sub & 4;
-  const uint32_t per_row = heads * nb;
-  const uint64_t items = static_cast<uint64_t>(rows) * per_row;
+  const int t = threadIdx.x & (kTeam - 1);
+  const uint32_t per_row = by_row.d, nb = kBlocks ? kBlocks : by_block.d;
+  const uint64_t items = static_cast<uint64_t>(rows) * per_row;  // (fewer than 2^32)
   const uint64_t teams = static_cast<uint64_t>(gridDim.x) * (kRowThreads / kTeam);
   for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kRowThreads / kTeam) + threadIdx.x / kTeam; item < items; item += teams) {
-    const uint32_t row = static_cast<uint32_t>(item / per_row);
-    const uint32_t rest = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * per_row);
-    const uint32_t head = rest / nb, b = rest - head * nb;
+    const uint32_t row = by_row.of(static_cast<uint32_t>(item)), rest = static_cast<uint32_t>(item) - row * per_row;
+    const uint32_t head = kBlocks ? rest / nb : by_block.of(rest), b = rest - head * nb;
     const int64_t slot = slots[row];
-    float kx[4] = {0.f, 0.f, 0.f, 0.f}, vx[4] = {0.f, 0.f, 0.f, 0.f};
+    float kx[8], vx[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      kx[e] = vx[e] = 0.0f;
     if (slot >= 0 && slot < capacity) {
-      const uint64_t page = static_cast<uint64_t>(slot) / page_tokens;
+      const uint64_t page = page_shift >= 0 ? slot >> page_shift : static_cast<uint64_t>(slot) / page_tokens;
       const uint32_t in_page = static_cast<uint32_t>(slot - page * page_tokens), token = in_page % kGroupTokens;
       const uint8_t *group = cache + page * page_stride +
                              static_cast<size_t>(head * (page_tokens / kGroupTokens) + in_page / kGroupTokens) * kv_group_bytes(32 * nb);
-      const uint32_t kq = *reinterpret_cast<const uint32_t *>(group + kv_key_word(nb, token, t, b)) >> shift;
-      const uint32_t vq = (*reinterpret_cast<const uint16_t *>(group + kv_value_half(nb, token, 2 * t, b)) |
-                           static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(group + kv_value_half(nb, token, 2 * t + 1, b))) << 16) >> shift;
+      const uint32_t kq = *reinterpret_cast<const uint32_t *>(group + kv_key_word(nb, token, t, b));
+      const uint32_t vq = *reinterpret_cast<const uint16_t *>(group + kv_value_half(nb, token, 2 * t, b)) |
+                          static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(group + kv_value_half(nb, token, 2 * t + 1, b))) << 16;
       const float kd = __half2float(*reinterpret_cast<const __half *>(group + kv_key_scale(nb, token, b)));
       const float vd = __half2float(*reinterpret_cast<const __half *>(group + kv_value_scale(nb, token, b)));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        kx[j] = __fmul_rn(kd, static_cast<float>(static_cast<int>((kq >> (8 * j)) & 15u) - 8));
-        vx[j] = __fmul_rn(vd, static_cast<float>(static_cast<int>((vq >> (8 * j)) & 15u) - 8));
+      for (int e = 0; e < 8; ++e) {
+        const int at = 8 * (e & 3) + (e & 4);
+        kx[e] = __fmul_rn(kd, static_cast<float>(static_cast<int>((kq >> at) & 15u) - 8));
+        vx[e] = __fmul_rn(vd, static_cast<float>(static_cast<int>((vq >> at) & 15u) - 8));
       }
     }
-    const size_t at = static_cast<size_t>(row) * per_row * 32 + rest * 32 + 4 * sub;
+    const size_t at = static_cast<size_t>(item) * 32 + 4 * t;
     store4(k + at, kx);
+    store4(k + at + 16, kx + 4);
     store4(v + at, vx);
+    store4(v + at + 16, vx + 4);
   }
 }
 
@@ -199,9 +212,11 @@ int store_rows(const RowTensor &k, const RowTensor &v, size_t rows, const int64_
   const uint32_t page_tokens = static_cast<uint32_t>(c.groups * kGroupTokens);
   const int64_t capacity = static_cast<int64_t>(c.pages) * page_tokens;
   const int grid = row_grid(static_cast<uint64_t>(rows) * heads * nb, 8);
-  auto *kernel = rows_aligned(k, sizeof(T)) && rows_aligned(v, sizeof(T)) ? kv_store_kernel<T, true> : kv_store_kernel<T, false>;
-  TCRV_CUDA_TRY(launch_pdl(kernel, grid, kRowThreads, 0, stream, k, v, slots, c.data, c.page_stride, capacity, page_tokens, heads,
-                           nb, static_cast<uint32_t>(rows)));
+  const bool vector = rows_aligned(k, sizeof(T)) && rows_aligned(v, sizeof(T));
+  auto *kernel = !vector ? kv_store_kernel<T, false, 0> : nb == 2 ? kv_store_kernel<T, true, 2> : nb == 4 ? kv_store_kernel<T, true, 4> : kv_store_kernel<T, true, 0>;
+  TCRV_CUDA_TRY(launch_pdl(kernel, grid, kRowThreads, 0, stream, k, v, slots, c.data, c.page_stride, capacity, page_tokens,
+                           shift_of(page_tokens), Divisor(heads * nb, static_cast<uint64_t>(rows) * heads * nb), Divisor(nb, heads * nb),
+                           static_cast<uint32_t>(rows)));
   return TCRV_CUDA_OK;
 }
 
@@ -211,8 +226,9 @@ int load_rows(void *k, void *v, size_t rows, const int64_t *slots, const tcrv_cu
   const uint32_t page_tokens = static_cast<uint32_t>(c.groups * kGroupTokens);
   const int64_t capacity = static_cast<int64_t>(c.pages) * page_tokens;
   const int grid = row_grid(static_cast<uint64_t>(rows) * heads * nb, 8);
-  TCRV_CUDA_TRY(launch_pdl(kv_load_kernel<T>, grid, kRowThreads, 0, stream, static_cast<T *>(k), static_cast<T *>(v), slots,
-                           static_cast<const uint8_t *>(c.data), c.page_stride, capacity, page_tokens, heads, nb,
+  TCRV_CUDA_TRY(launch_pdl(nb == 2 ? kv_load_kernel<T, 2> : nb == 4 ? kv_load_kernel<T, 4> : kv_load_kernel<T, 0>, grid, kRowThreads, 0, stream, static_cast<T *>(k), static_cast<T *>(v), slots,
+                           static_cast<const uint8_t *>(c.data), c.page_stride, capacity, page_tokens,
+                           shift_of(page_tokens), Divisor(heads * nb, static_cast<uint64_t>(rows) * heads * nb), Divisor(nb, heads * nb),
                            static_cast<uint32_t>(rows)));
   return TCRV_CUDA_OK;
 }

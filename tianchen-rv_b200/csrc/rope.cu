@@ -26,6 +26,7 @@ struct RopeParams {
   const double *freqs;
   float magnitude;
   bool wide_positions;
+  Divisor by_access, by_head;  // a head's accesses, a CTA's heads
 };
 
 // (cos, sin) of position * freq.  The product and its reduction to one turn are done in 64 bits: a
@@ -79,50 +80,98 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
   const uint32_t turning = kHalves ? pairs / kN : p.n_rot / (kN * kStep);
   const uint32_t per_head = turning + (p.dim - p.n_rot) / kN;
   const uint32_t items = ntok * nheads * per_head;
-  for (uint32_t i = threadIdx.x; i < items; i += kRopeThreads) {
-    const uint32_t row = i / per_head, a = i - row * per_head;
-    const uint32_t t = row / nheads, head = head0 + (row - t * nheads);
-    uint32_t w = 0;
+  // Two 16-byte loads to a thread before the first store, for 64 warps of one each do not cover the memory's latency
+  // (2047 tokens, half of each head of 128, f32: 43 us with one, 28 with two).  An item of the halves layout is two by itself
+  // and goes alone: two items cost the registers of a CTA (8192 tokens, bf16: 32 us with one, 44 with two).
+  if constexpr (kHalves) {
+    for (uint32_t i = threadIdx.x; i < items; i += kRopeThreads) {
+      const uint32_t row = p.by_access.of(i), a = i - row * per_head;
+      const uint32_t t = nheads == p.cta_heads ? p.by_head.of(row) : row / nheads, head = head0 + (row - t * nheads);
+      uint32_t w = 0;
 #pragma unroll
-    for (int j = 1; j < kRopeTensors; ++j)
-      w += j < p.count && head >= p.tensor[j].first_head;
-    const RopeTensor &tensor = p.tensor[w];
-    const size_t token = token0 + t, h = head - tensor.first_head;
-    const T *x = static_cast<const T *>(tensor.x) + token * tensor.x_token + h * tensor.x_head;
-    T *y = static_cast<T *>(tensor.y) + token * tensor.y_token + h * tensor.y_head;
-    const float2 *cs = rope_cs + t * pairs;
-    if (a >= turning) {
-      const uint32_t at = p.n_rot + (a - turning) * kN;
-      if (static_cast<const void *>(x) != static_cast<const void *>(y))
-        *reinterpret_cast<P *>(y + at) = *reinterpret_cast<const P *>(x + at);
-    } else if constexpr (kHalves) {
-      const P lo = *reinterpret_cast<const P *>(x + a * kN), hi = *reinterpret_cast<const P *>(x + pairs + a * kN);
-      P ylo, yhi;
+      for (int j = 1; j < kRopeTensors; ++j)
+        w += j < p.count && head >= p.tensor[j].first_head;
+      const RopeTensor &tensor = p.tensor[w];
+      const size_t token = token0 + t, h = head - tensor.first_head;
+      const T *x = static_cast<const T *>(tensor.x) + token * tensor.x_token + h * tensor.x_head;
+      T *y = static_cast<T *>(tensor.y) + token * tensor.y_token + h * tensor.y_head;
+      const float2 *cs = rope_cs + t * pairs;
+      if (a >= turning) {
+        const uint32_t at = p.n_rot + (a - turning) * kN;
+        if (tensor.x != tensor.y)
+          *reinterpret_cast<P *>(y + at) = *reinterpret_cast<const P *>(x + at);
+      } else {
+        const P lo = *reinterpret_cast<const P *>(x + a * kN), hi = *reinterpret_cast<const P *>(x + pairs + a * kN);
+        P ylo, yhi;
 #pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const float2 r = cs[a * kN + e];
-        const float u = to_float(lo.v[e]), v = to_float(hi.v[e]);
-        ylo.v[e] = from_float<T>(turn_lo(u, v, r));
-        yhi.v[e] = from_float<T>(turn_hi(u, v, r));
+        for (int e = 0; e < kN; ++e) {
+          const float2 r = cs[a * kN + e];
+          const float u = to_float(lo.v[e]), v = to_float(hi.v[e]);
+          ylo.v[e] = from_float<T>(turn_lo(u, v, r));
+          yhi.v[e] = from_float<T>(turn_hi(u, v, r));
+        }
+        *reinterpret_cast<P *>(y + a * kN) = ylo;
+        *reinterpret_cast<P *>(y + pairs + a * kN) = yhi;
       }
-      *reinterpret_cast<P *>(y + a * kN) = ylo;
-      *reinterpret_cast<P *>(y + pairs + a * kN) = yhi;
-    } else if constexpr (kN > 1) {
-      const P in = *reinterpret_cast<const P *>(x + a * kN);
-      P out;
+    }
+    return;
+  }
+  constexpr int kAtOnce = 2;
+  for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kAtOnce * kRopeThreads) {
+    P lo[kAtOnce], hi[kAtOnce];
+    T *to[kAtOnce];
+    const float2 *angle[kAtOnce];
+    bool turns[kAtOnce];
 #pragma unroll
-      for (int e = 0; e < kN; e += 2) {
-        const float2 r = cs[(a * kN + e) / 2];
-        const float u = to_float(in.v[e]), v = to_float(in.v[e + 1]);
-        out.v[e] = from_float<T>(turn_lo(u, v, r));
-        out.v[e + 1] = from_float<T>(turn_hi(u, v, r));
+    for (int k = 0; k < kAtOnce; ++k) {
+      const uint32_t i = i0 + k * kRopeThreads;
+      to[k] = nullptr;
+      if (i >= items)
+        continue;
+      const uint32_t row = p.by_access.of(i), a = i - row * per_head;
+      const uint32_t t = nheads == p.cta_heads ? p.by_head.of(row) : row / nheads, head = head0 + (row - t * nheads);
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 1; j < kRopeTensors; ++j)
+        w += j < p.count && head >= p.tensor[j].first_head;
+      const RopeTensor &tensor = p.tensor[w];
+      const size_t token = token0 + t, h = head - tensor.first_head;
+      turns[k] = a < turning;
+      const uint32_t at = turns[k] ? a * (kN * kStep) : p.n_rot + (a - turning) * kN;
+      const T *x = static_cast<const T *>(tensor.x) + token * tensor.x_token + h * tensor.x_head + at;
+      if (!turns[k] && tensor.x == tensor.y)
+        continue;
+      to[k] = static_cast<T *>(tensor.y) + token * tensor.y_token + h * tensor.y_head + at;
+      angle[k] = rope_cs + t * pairs + at / 2;
+      lo[k] = *reinterpret_cast<const P *>(x);
+      if (turns[k] && kN == 1)
+        hi[k] = *reinterpret_cast<const P *>(x + 1);
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (to[k] == nullptr)
+        continue;
+      if (turns[k]) {
+        if constexpr (kN == 1) {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) {
+            const float2 r = angle[k][e];
+            const float u = to_float(lo[k].v[e]), v = to_float(hi[k].v[e]);
+            lo[k].v[e] = from_float<T>(turn_lo(u, v, r));
+            hi[k].v[e] = from_float<T>(turn_hi(u, v, r));
+          }
+          *reinterpret_cast<P *>(to[k] + 1) = hi[k];
+        } else {
+#pragma unroll
+          for (int e = 0; e < kN; e += 2) {
+            const float2 r = angle[k][e / 2];
+            const float u = to_float(lo[k].v[e]), v = to_float(lo[k].v[e + 1]);
+            lo[k].v[e] = from_float<T>(turn_lo(u, v, r));
+            lo[k].v[e + 1] = from_float<T>(turn_hi(u, v, r));
+          }
+        }
       }
-      *reinterpret_cast<P *>(y + a * kN) = out;
-    } else {
-      const float2 r = cs[a];
-      const float u = to_float(x[2 * a]), v = to_float(x[2 * a + 1]);
-      y[2 * a] = from_float<T>(turn_lo(u, v, r));
-      y[2 * a + 1] = from_float<T>(turn_hi(u, v, r));
+      *reinterpret_cast<P *>(to[k]) = lo[k];
     }
   }
 }
@@ -177,6 +226,11 @@ int rope_launch(RopeParams &p, bool halves, bool inverse, cudaStream_t stream) {
   p.cta_tokens = static_cast<uint32_t>(tokens);
   p.cta_heads = static_cast<uint32_t>((p.heads + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(ctas), (p.heads + p.cta_heads - 1) / p.cta_heads);
+  const uint32_t n = wide ? kN : 1, step = halves ? 1 : wide ? 1 : 2;
+  const uint32_t accesses = (halves ? pairs / n : p.n_rot / (n * step)) + (p.dim - p.n_rot) / n;
+  const uint64_t rows = static_cast<uint64_t>(p.cta_tokens) * p.cta_heads;
+  p.by_access = Divisor(accesses, rows * accesses);
+  p.by_head = Divisor(p.cta_heads, rows);
   const size_t smem = tokens * pairs * sizeof(float2);
   auto *kernel = halves ? (wide ? rope_kernel_of<T, true, kN>(inverse) : rope_kernel_of<T, true, 1>(inverse))
                         : (wide ? rope_kernel_of<T, false, kN>(inverse) : rope_kernel_of<T, false, 1>(inverse));

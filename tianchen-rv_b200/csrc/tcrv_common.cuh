@@ -88,6 +88,16 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int block, si
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+// Division of 32-bit numbers below `limit` by a divisor that a kernel gets as an argument: one multiplication where
+// ceil(2^32 / d) is exact enough (n d < 2^32), the division elsewhere.
+struct Divisor {
+  uint32_t d, magic;  // magic 0: divide
+  Divisor() = default;
+  Divisor(uint32_t divisor, uint64_t limit)
+      : d(divisor), magic(divisor > 1 && limit * divisor < (1ull << 32) ? static_cast<uint32_t>((1ull << 32) / divisor + ((1ull << 32) % divisor != 0)) : 0) {}
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return magic != 0 ? __umulhi(n, magic) : n / d; }
+};
+
 __device__ __forceinline__ float half_bits_to_float(uint32_t bits16) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }
