@@ -38,8 +38,8 @@ struct ColumnParams {
 
 // What the combine step has to know of the context range that begins in CTA c and ends in a later one.
 struct SplitRange {
-  int32_t valid, request, head, column_group, last_cta;
-  int32_t pad[3];
+  int32_t valid, head, column_group, last_cta, rows, first_row;
+  int32_t pad[2];
 };
 
 // Workspace: one SplitRange per CTA, then (maximum, sum) and the accumulators of two partial ranges per
@@ -333,8 +333,13 @@ __device__ __forceinline__ void write_row(const tcrv_cuda_attention_call &c, siz
 // CTA of equal length, whatever the contexts' lengths; inside a range the warps take units in turn, each
 // with a ring of its own that its first two lanes fill by bulk copies ahead of use, across segment ends.  A
 // segment that lies in one range is finished there; of one that does not, each CTA leaves maximum, sum and
-// accumulators in the workspace for the combine kernel.  Bound by bytes at decode (9/16 byte a value, used
-// for at most 8 NT columns), with the instructions that unpack them next: about 500 for a warp's unit.
+// accumulators in the workspace for the combine kernel.
+//
+// Bound by instructions, not by the 9/16 byte a value: a warp's unit of D = 128 and 8 rows takes about 880 (32 words unpacked
+// at 9 each, 32 products, the weights of each block, the soft-max, the copies' addresses), issued in 59 % of the cycles by 16
+// warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 89 us, 3.4 TB/s of cache; with (w & mask) | bits left to the compiler as two
+// instructions, products that add to zeroed registers, and 64-bit cursors, 1100 instructions and 112 us.  Rows of several
+// tiles share a unit's unpacking (NT); their accumulators leave room for one CTA of 8 warps on an SM from 16 rows of 128 on.
 template <int NB, int NT, int TERMS>
 __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(const __grid_constant__ ColumnParams p) {
   using L = ColumnLayout<NB, NT, TERMS>;
@@ -512,7 +517,13 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     for (; u < to; u += kWarps) {
       if (!failed && !mbar_wait_bounded(&bars[stage], parity)) {
         failed = true;
-        raise_device_error(p.errors, kDevErrBarrierTimeout);
+        if (lane == 0)
+          raise_device_error(p.errors, kDevErrBarrierTimeout);
+        // no further copy; those on their way are waited for, with the same limit
+        for (int s = 1; s < kStages && u + s * kWarps < units; ++s)
+          mbar_wait_bounded(&bars[(stage + s) % kStages], parity ^ (stage + s >= kStages ? 1u : 0u));
+        mbar_wait_bounded(&bars[stage], parity);
+        next = units;
       }
       const uint8_t *unit = ring + stage * L::kUnitBytes;
       const uint32_t there = flags[stage];
@@ -783,7 +794,8 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     if (threadIdx.x == 0 && to == units) {
       SplitRange range = {};
       range.valid = !first && seg_end > units;
-      range.request = static_cast<int32_t>(at.r);
+      range.rows = at.q.rows;
+      range.first_row = at.q.first_row;
       range.head = head;
       range.column_group = column_group;
       if (range.valid) {  // the CTA that holds the segment's last unit
@@ -814,10 +826,9 @@ __global__ void __launch_bounds__(kCombineThreads) columns_combine_kernel(const 
   const SplitRange range = static_cast<const SplitRange *>(c.workspace)[blockIdx.x];
   if (!range.valid)
     return;
-  const Request q = load_request(p, range.request, rows);
   const float *stats = reinterpret_cast<const float *>(ws + column_stats_offset(gridDim.x));
   const float *sums = reinterpret_cast<const float *>(ws + column_sums_offset(gridDim.x, rows));
-  const int32_t pair0 = range.column_group * rows, pairs = min(rows, q.rows * static_cast<int32_t>(p.group) - pair0);
+  const int32_t pair0 = range.column_group * rows, pairs = min(rows, range.rows * static_cast<int32_t>(p.group) - pair0);
   const int parts = range.last_cta - static_cast<int>(blockIdx.x) + 1;
   // part i: the second slot of the first CTA, the first slots of the others
   auto slot = [&](int i) { return 2 * static_cast<size_t>(blockIdx.x + i) + (i == 0 ? 1 : 0); };
@@ -855,7 +866,7 @@ __global__ void __launch_bounds__(kCombineThreads) columns_combine_kernel(const 
     for (int k = 0; k * kCombineThreads < kDim; ++k) {
       const int d = threadIdx.x + k * kCombineThreads;
       if (d < kDim)
-        write_row(c, q.first_row + token, range.head * p.group + (pair - token * p.group), d, sum[k], total, top);
+        write_row(c, range.first_row + token, range.head * p.group + (pair - token * p.group), d, sum[k], total, top);
     }
     __syncthreads();
   }

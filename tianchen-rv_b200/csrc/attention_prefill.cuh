@@ -7,6 +7,12 @@
 // Warps 0..7 are the soft-max, of one tile after the other: two threads to a row, 64 columns each; warps 8..15 turn quants into the fp16
 // operands in shared memory, warp 16 issues the products.  While one tile's soft-max runs the other tile's products do.
 //
+// What bounds it: the soft-max warps, which never wait (a step of one tile takes them about 2100 cycles, 1024 of them the
+// exponential unit's; the tensor cores are busy 35 to 40 % of the time).  4 prompts of up to 2048 tokens behind contexts of up to
+// 2048, 32 / 8 heads of 128, bf16: 453 us, 675 TFLOP/s of the pairs that count.  Measured on the way: four warps unpacking instead
+// of eight 818 us; a thread to a row, one warpgroup to a tile, 459 (with the tiles' passes taking turns 510); half of the
+// exponentials by a polynomial 517, for the schedulers have no cycles to spare for it.
+//
 // Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
 // scaled block by block without reading S and O once for every block of 32.  Query rows are fp16 after a power of two
 // (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A group with a scale so large that
@@ -60,7 +66,7 @@ struct PrefillLayout {
   static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
   static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group]: tokens with a value scale that is no number
   static constexpr int kBars = kPoison + kSlots * kTileGroups * 2;
-  static constexpr int kBarCount = 19;
+  static constexpr int kBarCount = 20;
   static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
   static constexpr int kTmem = kTops + 2 * 2 * 128 * 4;
   static constexpr int kAbort = kTmem + 4;
@@ -68,7 +74,7 @@ struct PrefillLayout {
 };
 
 // barriers
-enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15 };
+enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15, kBarDrain = 19 };
 
 // kind::f16, fp16 A and B (both K-major), f32 D.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
@@ -199,6 +205,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     }
     for (int i = 0; i < 4; ++i)
       mbar_init(&bars[kBarPair + i], 2);
+    mbar_init(&bars[kBarDrain], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -749,6 +756,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         }
         __syncwarp();
       }
+    }
+    if (!good) {  // products on their way end before their memory goes back
+      if (leader)
+        umma_commit(&bars[kBarDrain]);
+      __syncwarp();
+      mbar_wait_bounded(&bars[kBarDrain], 0);
     }
     }
   }
