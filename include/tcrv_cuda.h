@@ -474,7 +474,8 @@ int tcrv_cuda_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_
  * more than `width` pages), 3 (more than `rows` rows), 4 (a negative length, or a free count that is
  * negative or more than free_capacity) - the last one that applies -, first_rows and row counts are 0,
  * slots are -1, kv_lens are context_lens and the block table stays.  free_count may be info + 3 of an
- * earlier call, also of this one's info. */
+ * earlier call, also of this one's info, and kv_lens may be context_lens; no other output may overlap
+ * an input. */
 typedef struct {
   size_t requests, page_tokens, width, rows, free_capacity;
   const int32_t *context_lens, *new_lens;

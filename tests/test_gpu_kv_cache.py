@@ -205,6 +205,26 @@ def test_plan_in_a_captured_loop(cuda, pkg):
         assert np.array_equal(table.cpu().numpy(), want_table)
 
 
+@pytest.mark.parametrize("n", [7, 3000])
+def test_plan_that_replaces_its_own_inputs(cuda, pkg, n):
+    # the lengths and the free count of one step are the next one's, in the same buffers
+    rng = np.random.default_rng(n)
+    ints = lambda x: cuda.tensor(x, dtype=cuda.int32, device="cuda")  # noqa: E731
+    width, rows = 8, 4 * n
+    state, left, table = [0] * n, 8 * n, np.full((n, width), -1, np.int32)
+    free = [int(x) for x in rng.permutation(8 * n)]
+    t, f = ints(table), ints(free)
+    plan = pkg.kv_plan(ints(state), ints(state), t, f, ints([left]), 16, rows)
+    for step in range(6):
+        new = [int(x) for x in rng.integers(0, 5, n)] if step != 3 else [200] * n  # (once what cannot be done)
+        pkg.kv_plan(plan.kv_lens, ints(new), t, f, plan.info[3:4], 16, rows, out=plan)
+        want, table = ref.plan(state, new, table, free, left, 16, rows)
+        for x, w in zip(plan, want):
+            assert np.array_equal(x.cpu().numpy(), w)
+        assert np.array_equal(t.cpu().numpy(), table)
+        state, left = [int(x) for x in want[1]], int(want[5][3])
+
+
 def test_plan_refusals(cuda, pkg):
     ints = lambda x: cuda.tensor(x, dtype=cuda.int32, device="cuda")  # noqa: E731
     ok = [ints([1, 2]), ints([1, 1]), ints([[0, 1], [2, 3]]), ints([4]), ints([1]), 16, 2]

@@ -616,7 +616,7 @@ def kv_plan(context_lens, new_lens, block_table, free_pages, free_count, page_to
     taken, pages left).  A step that cannot be done has a status other than 0, takes nothing and has no
     rows: 1 too few free pages, 2 more than `width` pages to a request, 3 more than `rows` rows, 4 a
     negative length or an impossible free count.  All int32 but the slots (int64).  `out`, an earlier
-    plan of the same sizes, is overwritten; `free_count` may be its info[3:4]."""
+    plan of the same sizes, is overwritten; `free_count` may be its info[3:4] and `context_lens` its kv_lens."""
     return KvPlan(_native.kv_plan(context_lens, new_lens, block_table, free_pages, free_count, page_tokens, rows, out))
 
 

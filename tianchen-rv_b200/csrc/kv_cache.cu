@@ -295,14 +295,14 @@ __device__ __forceinline__ uint32_t plan_find(const int32_t *first, uint32_t n, 
 // Every CTA sums all requests (their two prefix sums stay in its shared memory), then the CTAs deal
 // out the requests, the new pages and the rows among themselves; which request a page or row belongs
 // to is found by bisection, so a step of one long prompt is as even as one of many tokens.  The cluster
-// is there for the free count: it may be an input that this call's info replaces, so it is written
-// only when all CTAs have read it.  Bound by latency: two dependent global reads, the scan, one write.
+// is there for inputs that outputs may replace (the free count, the lengths): nothing is written before all CTAs
+// have read them.  Bound by latency: two dependent global reads, the scan, one write.
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(tcrv_cuda_kv_plan_call c) {
   extern __shared__ int32_t plan_smem[];
   __shared__ PlanSums warp_sums[32];
   __shared__ int bad;
   const uint32_t n = static_cast<uint32_t>(c.requests), page = static_cast<uint32_t>(c.page_tokens);
-  int32_t *first_row = plan_smem, *first_page = plan_smem + n + 1;
+  int32_t *first_row = plan_smem, *first_page = first_row + n + 1, *context = first_page + n + 1;
   if (threadIdx.x == 0)
     bad = 0;
   pdl_enter();
@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(tcrv_cuda_kv_plan
     if (r < n) {  // (a sum beyond 31 bits is refused below)
       first_row[r] = static_cast<int32_t>(base.rows + at.rows);
       first_page[r] = static_cast<int32_t>(base.pages + at.pages);
+      context[r] = c.context_lens[r];
     }
     base.rows += total.rows;
     base.pages += total.pages;
@@ -350,16 +351,18 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(tcrv_cuda_kv_plan
     status = 4;
   const bool ok = status == 0;
 
+  if (gridDim.x > 1)
+    cooperative_groups::this_cluster().sync();  // (kv_lens may be context_lens, info[3] the free count: all have read them)
   const uint32_t threads = gridDim.x * kPlanThreads, tid = blockIdx.x * kPlanThreads + threadIdx.x;
   for (uint32_t r = tid; r <= n; r += threads) {
     c.first_rows[r] = ok ? first_row[r] : 0;
     if (r < n)
-      c.kv_lens[r] = ok ? c.context_lens[r] + c.new_lens[r] : c.context_lens[r];
+      c.kv_lens[r] = ok ? context[r] + (first_row[r + 1] - first_row[r]) : context[r];
   }
   if (ok) {
     for (uint32_t j = tid; j < static_cast<uint32_t>(base.pages); j += threads) {
       const uint32_t r = plan_find(first_page, n, static_cast<int32_t>(j));
-      const uint32_t held = (static_cast<uint32_t>(c.context_lens[r]) + page - 1) / page;
+      const uint32_t held = (static_cast<uint32_t>(context[r]) + page - 1) / page;
       c.block_table[r * c.table_stride + held + (j - first_page[r])] = c.free_pages[free_count - 1 - j];
     }
   }
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(tcrv_cuda_kv_plan
     int32_t position = 0, request = -1;
     if (i < used) {
       const uint32_t r = plan_find(first_row, n, static_cast<int32_t>(i));
-      const uint32_t ctx = static_cast<uint32_t>(c.context_lens[r]), held = (ctx + page - 1) / page;
+      const uint32_t ctx = static_cast<uint32_t>(context[r]), held = (ctx + page - 1) / page;
       const uint32_t p = ctx + (static_cast<uint32_t>(i) - first_row[r]), at = p / page;
       const int32_t id = at < held ? c.block_table[r * c.table_stride + at]
                                    : c.free_pages[free_count - 1 - (first_page[r] + (at - held))];
@@ -381,10 +384,6 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(tcrv_cuda_kv_plan
     c.positions[i] = position;
     c.row_requests[i] = request;
   }
-  if (gridDim.x > 1)
-    cooperative_groups::this_cluster().sync();
-  else
-    __syncthreads();
   if (tid == 0) {
     c.info[0] = status;
     c.info[1] = static_cast<int32_t>(used);
@@ -416,7 +415,7 @@ int launch_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *
 }
 
 int launch_kv_plan(const tcrv_cuda_kv_plan_call &call, cudaStream_t stream) {
-  const size_t smem = (2 * call.requests + 2) * sizeof(int32_t);
+  const size_t smem = (3 * call.requests + 2) * sizeof(int32_t);
   if (smem > 48 * 1024)
     TCRV_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   const bool alone = call.requests <= kPlanAlone && call.rows <= kPlanAlone;
