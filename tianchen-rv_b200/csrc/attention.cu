@@ -16,7 +16,7 @@ constexpr size_t kPrefillRows = 33;
 
 struct Shape {
   // the columns kernel
-  int tiles, terms, rows;  // rows: query rows of a column group, 8 to a tile
+  int tiles, mode, rows;  // rows: query rows of a column group, 8 to a tile (4 of kPairs)
   int grid;
   long long most_rows;
   // the prefill kernel
@@ -29,7 +29,6 @@ struct Shape {
 Shape shape_of(const tcrv_cuda_attention_call &c) {
   Shape s = {};
   const size_t group = c.heads / c.cache.kv_heads, all = c.max_new * group;
-  s.terms = c.type == TCRV_CUDA_TYPE_F32 ? 2 : 1;
   s.prefill = all >= kPrefillRows && c.type != TCRV_CUDA_TYPE_F32 && (c.cache.dim == 64 || c.cache.dim == 128);
   const size_t rows = s.prefill ? kPrefillRows - 1 : all;
   s.most_rows = static_cast<long long>(rows);
@@ -37,7 +36,8 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   const size_t most_rows = 8 * (c.cache.dim <= 64 ? 4 : c.cache.dim <= 128 ? 3 : c.cache.dim <= 192 ? 2 : 1);
   const size_t groups = (rows + most_rows - 1) / most_rows;
   s.tiles = static_cast<int>(((rows + groups - 1) / groups + 7) / 8);
-  s.rows = 8 * s.tiles;
+  s.mode = c.type != TCRV_CUDA_TYPE_F32 ? kOneTerm : rows <= 4 ? kPairs : kTwoTerms;
+  s.rows = s.mode == kPairs ? 4 : 8 * s.tiles;
   const size_t units = (c.width * c.cache.groups + kUnitGroups - 1) / kUnitGroups;
   const double most = static_cast<double>(units ? units : 1) * groups * c.cache.kv_heads * c.requests / kWarps + 1;
   const int cap = sm_count() * ctas_per_sm(static_cast<int>(c.cache.dim / 32), s.tiles);
@@ -81,10 +81,10 @@ int configure(Configured &state, const void *kernel, size_t smem, int threads, i
   return TCRV_CUDA_OK;
 }
 
-template <int NB, int NT, int TERMS>
+template <int NB, int NT, int MODE>
 int launch_columns(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
-  constexpr size_t smem = ColumnLayout<NB, NT, TERMS>::kBytes;
-  auto *kernel = columns_kernel<NB, NT, TERMS>;
+  constexpr size_t smem = ColumnLayout<NB, NT, MODE>::kBytes;
+  auto *kernel = columns_kernel<NB, NT, MODE>;
   static Configured state;
   const int st = configure(state, reinterpret_cast<const void *>(kernel), smem, kThreads, 0);
   if (st != TCRV_CUDA_OK)
@@ -97,22 +97,22 @@ int launch_columns(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
   return TCRV_CUDA_OK;
 }
 
-template <int NB, int TERMS>
+template <int NB, int MODE>
 int launch_tiles(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
   switch (s.tiles) {
     case 1:
-      return launch_columns<NB, 1, TERMS>(p, s, stream);
+      return launch_columns<NB, 1, MODE>(p, s, stream);
     case 2:
       if constexpr (NB <= 6)
-        return launch_columns<NB, 2, TERMS>(p, s, stream);
+        return launch_columns<NB, 2, MODE>(p, s, stream);
       break;
     case 3:
       if constexpr (NB <= 4)
-        return launch_columns<NB, 3, TERMS>(p, s, stream);
+        return launch_columns<NB, 3, MODE>(p, s, stream);
       break;
     case 4:
       if constexpr (NB <= 2)
-        return launch_columns<NB, 4, TERMS>(p, s, stream);
+        return launch_columns<NB, 4, MODE>(p, s, stream);
       break;
   }
   return TCRV_CUDA_ERR_UNSUPPORTED;
@@ -120,7 +120,9 @@ int launch_tiles(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
 
 template <int NB>
 int launch_dim(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
-  return s.terms == 1 ? launch_tiles<NB, 1>(p, s, stream) : launch_tiles<NB, 2>(p, s, stream);
+  return s.mode == kOneTerm ? launch_tiles<NB, kOneTerm>(p, s, stream)
+         : s.mode == kPairs ? launch_columns<NB, 1, kPairs>(p, s, stream)
+                            : launch_tiles<NB, kTwoTerms>(p, s, stream);
 }
 
 template <int NB>

@@ -11,7 +11,8 @@
 // multiplies the soft-max weight, one operand per block.  What is rounded is the query row (scaled by a
 // power of two so that its largest element lies in [2^14, 2^15)) and the weight times the value's scale:
 //   fp16 and bf16 calls: both to one fp16 term, 2^-12 relative (a 16-bit query is exact);
-//   f32 calls: both to two fp16 terms, 2^-22 relative, with a product each into the same sums.  The value
+//   f32 calls: both to two fp16 terms, 2^-22 relative, with a product each into the same sums, or up to 4
+//   rows with a column each (777 tokens, 4 rows: 19 us against 15).  The value
 //   scales are lifted by a power of two that follows the largest one seen, like the running maximum.
 // Maximum, sum and accumulators are f32.
 #pragma once
@@ -54,17 +55,22 @@ inline size_t column_workspace_bytes(size_t ctas, size_t rows, size_t dim) {
 
 inline int ctas_per_sm(int nb, int nt) { return nb * nt <= 4 ? 2 : 1; }
 
-template <int NB, int NT, int TERMS>
+// How a call's numbers become fp16 operands.
+constexpr int kOneTerm = 1;   // fp16 and bf16
+constexpr int kTwoTerms = 2;  // f32: two products into the same sums
+constexpr int kPairs = 3;     // f32, up to 4 rows: the terms in neighbouring columns of the one tile, which has room for them
+
+template <int NB, int NT, int MODE>
 struct ColumnLayout {
   static constexpr int kDim = 32 * NB;
   static constexpr int kStages = NB * NT <= 2 ? 4 : NB * NT <= 3 ? 3 : NB >= 6 ? 2 : NB * NT > 4 ? 4 : 2;  // (what shared memory has room for)
   static constexpr int kUnitBytes = kUnitGroups * 18 * kDim;
-  static constexpr int kTileRows = 8;            // query rows of a tile
+  static constexpr int kTileRows = MODE == kPairs ? 4 : 8;  // query rows of a tile
   static constexpr int kRows = NT * kTileRows;   // of a column group
   static constexpr int kSums = kStages * kWarps * kUnitBytes;                     // f32 [warp][row of a tile][d]
   static constexpr int kQuery = kSums + kWarps * kTileRows * kDim * 4;            // fp16 operand of the rows
   static constexpr int kQueryBytes = NT * NB * 512;                               // of a term
-  static constexpr int kStats = kQuery + TERMS * kQueryBytes;                     // f32 [warp][row][max, sum]
+  static constexpr int kStats = kQuery + (MODE == kTwoTerms ? 2 : 1) * kQueryBytes;                     // f32 [warp][row][max, sum]
   static constexpr int kRowInfo = kStats + kWarps * kRows * 2 * 4;                // f32 scale, int position
   static constexpr int kFlags = kRowInfo + kRows * 8;                             // u32 [stage][warp]
   static constexpr int kBars = (kFlags + kStages * kWarps * 4 + 7) / 8 * 8;
@@ -340,11 +346,12 @@ __device__ __forceinline__ void write_row(const tcrv_cuda_attention_call &c, siz
 // warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 89 us, 3.4 TB/s of cache; with (w & mask) | bits left to the compiler as two
 // instructions, products that add to zeroed registers, and 64-bit cursors, 1100 instructions and 112 us.  Rows of several
 // tiles share a unit's unpacking (NT); their accumulators leave room for one CTA of 8 warps on an SM from 16 rows of 128 on.
-template <int NB, int NT, int TERMS>
+template <int NB, int NT, int MODE>
 __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(const __grid_constant__ ColumnParams p) {
-  using L = ColumnLayout<NB, NT, TERMS>;
+  using L = ColumnLayout<NB, NT, MODE>;
   constexpr int kDim = L::kDim, kStages = L::kStages, kGroupBytes = 18 * kDim, kRows = L::kRows, kTileRows = L::kTileRows;
-  constexpr int kMine = 2;  // query rows of a tile that a lane has
+  constexpr int kMine = MODE == kPairs ? 1 : 2;  // query rows of a tile that a lane has
+  const auto row_of = [](int t, int i) { return MODE == kPairs ? t : 2 * t + i; };
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long scratch[kWarps];
   __shared__ Cursor start;
@@ -445,6 +452,8 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
       const int i = k * kWarps + warp;
+      if (MODE == kPairs && i >= kRows)
+        break;
       float top = 0.0f;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -461,10 +470,10 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       for (int b = 0; b < NB; ++b) {
         const float v = row_values[k][b] * lift;
         const __half hi = __float2half_rn(v);
-        const int place = (((k * NB + b) * 32 + warp * 4 + (f >> 2)) * 4 + kstep * 2 + (f & 1)) * 2 + ((f & 2) >> 1);
+        const int place = (((k * NB + b) * 32 + (MODE == kPairs ? 2 : 1) * warp * 4 + (f >> 2)) * 4 + kstep * 2 + (f & 1)) * 2 + ((f & 2) >> 1);
         operand[place] = hi;
-        if constexpr (TERMS == 2)
-          operand[place + L::kQueryBytes / 2] = isfinite(v) ? __float2half_rn(v - __half2float(hi)) : __float2half_rn(0.0f);
+        if constexpr (MODE != kOneTerm)  // (pairs: the column after it, four lanes on)
+          operand[place + (MODE == kPairs ? 4 * 8 : L::kQueryBytes / 2)] = isfinite(v) ? __float2half_rn(v - __half2float(hi)) : __float2half_rn(0.0f);
       }
       if (lane == 0) {
         row_scale[i] = c.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
@@ -491,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int row = j * kTileRows + 2 * t + i;
+        const int row = j * kTileRows + row_of(t, i);
         scale[j][i] = row_scale[row];
         position[j][i] = row_position[row];
       }
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
             float acc[4];
             mma16816_zero(acc, a0, q.x, q.y);
             mma16816(acc, a1, q.z, q.w);
-            if constexpr (TERMS == 2) {
+            if constexpr (MODE == kTwoTerms) {
               const uint4 low = *reinterpret_cast<const uint4 *>(smem + L::kQuery + L::kQueryBytes + ((j * NB + b) * 32 + lane) * 16);
               mma16816(acc, a0, low.x, low.y);
               mma16816(acc, a1, low.z, low.w);
@@ -581,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           for (int gr = 0; gr < kUnitGroups; ++gr)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float v = s[gr][j][2 * h + i] * scale[j][i];
+              float v = (MODE == kPairs ? s[gr][j][2 * h] + s[gr][j][2 * h + 1] : s[gr][j][2 * h + i]) * scale[j][i];
               if (!whole) {
                 const int32_t token = token0 + gr * kGroupTokens + h * 8 + g;
                 if (!((there >> gr) & 1u) || token > position[j][i] || (window && token <= position[j][i] - window))
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           }
         }
       float lift = 1.0f, relift = 1.0f;
-      if constexpr (TERMS == 2) {
+      if constexpr (MODE != kOneTerm) {
         const auto largest = [&](bool finite_only) {
           __half2 most = __float2half2_rn(0.0f);
 #pragma unroll
@@ -660,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const float f0 = alpha[j][0] * relift, f1 = alpha[j][1] * relift;
+            const float f0 = alpha[j][0] * relift, f1 = alpha[j][kMine - 1] * relift;
             o[i][j][0] *= f0;
             o[i][j][1] *= f1;
             o[i][j][2] *= f0;
@@ -681,24 +690,33 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           const uint32_t a1[4] = {high_nibbles(w0[b]), high_nibbles(w0[b] >> 8), high_nibbles(w1[b]), high_nibbles(w1[b] >> 8)};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            uint32_t bits[TERMS][2];
+            constexpr int kProducts = MODE == kTwoTerms ? 2 : 1;
+            uint32_t bits[kProducts][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float d = TERMS == 2 ? scale_of(vd[gr][h], b) * lift : scale_of(vd[gr][h], b);
-              float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][1]), make_float2(d, d));
-              if (!whole) {  // a weight of zero stays zero, whatever the scale
-                x.x = pr[gr][j][h][0] == 0.0f ? 0.0f : x.x;
-                x.y = pr[gr][j][h][1] == 0.0f ? 0.0f : x.y;
-              }
-              const __half2 hi = __floats2half2_rn(x.x, x.y);
-              bits[0][h] = transpose8x8(half2_bits(hi));
-              if constexpr (TERMS == 2) {
-                const float2 y = __half22float2(hi);
-                bits[1][h] = transpose8x8(half2_bits(__floats2half2_rn(x.x - y.x, x.y - y.y)));
+              const float d = MODE == kOneTerm ? scale_of(vd[gr][h], b) : scale_of(vd[gr][h], b) * lift;
+              if constexpr (MODE == kPairs) {
+                float v = pr[gr][j][h][0] * d;
+                if (!whole)
+                  v = pr[gr][j][h][0] == 0.0f ? 0.0f : v;
+                const float hi = __half2float(__float2half_rn(v));
+                bits[0][h] = transpose8x8(half2_bits(__floats2half2_rn(hi, v - hi)));
+              } else {
+                float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][kMine - 1]), make_float2(d, d));
+                if (!whole) {  // a weight of zero stays zero, whatever the scale
+                  x.x = pr[gr][j][h][0] == 0.0f ? 0.0f : x.x;
+                  x.y = pr[gr][j][h][kMine - 1] == 0.0f ? 0.0f : x.y;
+                }
+                const __half2 hi = __floats2half2_rn(x.x, x.y);
+                bits[0][h] = transpose8x8(half2_bits(hi));
+                if constexpr (MODE == kTwoTerms) {
+                  const float2 y = __half22float2(hi);
+                  bits[kProducts - 1][h] = transpose8x8(half2_bits(__floats2half2_rn(x.x - y.x, x.y - y.y)));
+                }
               }
             }
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
+            for (int term = 0; term < kProducts; ++term) {
               mma16816(o[2 * b][j], a0, bits[term][0], bits[term][1]);
               mma16816(o[2 * b + 1][j], a1, bits[term][0], bits[term][1]);
             }
@@ -727,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         for (int off = 4; off <= 16; off <<= 1)
           l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], off);
         if (g == 0)
-          stats[(warp * kRows + j * kTileRows + 2 * t + i) * 2] = m[j][i];
+          stats[(warp * kRows + j * kTileRows + row_of(t, i)) * 2] = m[j][i];
       }
     __syncthreads();
     const bool first = seg_begin < 0, split = first || seg_end > units;
@@ -741,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       float f[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int row = j * kTileRows + 2 * t + i;
+        const int row = j * kTileRows + row_of(t, i);
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
@@ -749,15 +767,19 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         f[i] = m[j][i] == -INFINITY ? 0.0f : exp2_fast(m[j][i] - top);
         if (g == 0)
           stats[(warp * kRows + row) * 2 + 1] = l[j][i] * f[i];
-        if constexpr (TERMS == 2)
+        if constexpr (MODE != kOneTerm)
           f[i] *= lifted > -100 ? exp2f(static_cast<float>(lifted - 14)) : 1.0f;
       }
       float *mine = sums + warp * kTileRows * kDim;
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) {
         const int d = (i >> 1) * 32 + (i & 1) * 16 + 2 * g;
-        *reinterpret_cast<float2 *>(mine + 2 * t * kDim + d) = make_float2(o[i][j][0] * f[0], o[i][j][2] * f[0]);
-        *reinterpret_cast<float2 *>(mine + (2 * t + 1) * kDim + d) = make_float2(o[i][j][1] * f[1], o[i][j][3] * f[1]);
+        if constexpr (MODE == kPairs) {
+          *reinterpret_cast<float2 *>(mine + t * kDim + d) = make_float2((o[i][j][0] + o[i][j][1]) * f[0], (o[i][j][2] + o[i][j][3]) * f[0]);
+        } else {
+          *reinterpret_cast<float2 *>(mine + 2 * t * kDim + d) = make_float2(o[i][j][0] * f[0], o[i][j][2] * f[0]);
+          *reinterpret_cast<float2 *>(mine + (2 * t + 1) * kDim + d) = make_float2(o[i][j][1] * f[kMine - 1], o[i][j][3] * f[kMine - 1]);
+        }
       }
       __syncthreads();
       for (int i = threadIdx.x; i < kTileRows * kDim; i += kThreads) {
