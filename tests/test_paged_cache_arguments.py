@@ -56,6 +56,8 @@ def test_rope_arguments(pkg):
         assert call(**bad) == INVALID, bad
     assert call(dim=8192) == UNSUPPORTED and call(tokens=1 << 40) == UNSUPPORTED
     assert call(tensors=RopeTensor(A, A, 1 << 20)) == UNSUPPORTED
+    many = (RopeTensor * 4)(*[RopeTensor(A, A, 65535) for _ in range(4)])
+    assert call(tensors=many, count=4, dim=4096) == UNSUPPORTED
     assert call(tokens=0) == OK and call(count=0) == OK and call(tensors=RopeTensor(None, None, 0)) == OK
     def freqs(n=64, base=1e4, scaling=0, factor=1.0, original=0.0, low=1.0, high=32.0, out=A):
         return L.tcrv_cuda_rope_frequencies_f64(n, base, scaling, factor, original, low, high, out, None)

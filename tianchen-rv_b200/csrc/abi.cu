@@ -684,6 +684,8 @@ int tcrv_cuda_rope_rows(int type, size_t tokens, size_t dim, size_t n_rot, const
   }
   if (heads == 0)
     return TCRV_CUDA_OK;
+  if (heads * dim > (1u << 28))  // (a CTA counts the accesses of four tokens in 32 bits)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
   if (!positions || (n_rot != 0 && !freqs))
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
   return launch_rope_rows(type, tokens, dim, n_rot, tensors, count, positions, freqs, magnitude, flags, as_stream(stream));

@@ -28,7 +28,7 @@ struct Shape {
 
 Shape shape_of(const tcrv_cuda_attention_call &c) {
   Shape s = {};
-  const size_t group = c.heads / c.cache.kv_heads, all = c.max_new * group;
+  const size_t group = c.heads / c.cache.kv_heads, all = (c.max_new < c.rows ? c.max_new : c.rows) * group;
   s.prefill = all >= kPrefillRows && c.type != TCRV_CUDA_TYPE_F32 && (c.cache.dim == 64 || c.cache.dim == 128);
   const size_t rows = s.prefill ? kPrefillRows - 1 : all;
   s.most_rows = static_cast<long long>(rows);
