@@ -39,7 +39,7 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   s.mode = c.type != TCRV_CUDA_TYPE_F32 ? kOneTerm : rows <= 4 ? kPairs : kTwoTerms;
   s.rows = s.mode == kPairs ? 4 : 8 * s.tiles;
   const size_t units = (c.width * c.cache.groups + kUnitGroups - 1) / kUnitGroups;
-  const double most = static_cast<double>(units ? units : 1) * groups * c.cache.kv_heads * c.requests / kWarps + 1;
+  const double most = static_cast<double>((units ? units : 1) + kSegmentUnits) * groups * c.cache.kv_heads * c.requests / kWarps + 1;
   const int cap = sm_count() * ctas_per_sm(static_cast<int>(c.cache.dim / 32), s.tiles);
   s.grid = most < cap ? static_cast<int>(most) : cap;
   s.columns_bytes = column_workspace_bytes(s.grid, s.rows, c.cache.dim);

@@ -28,6 +28,9 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kUnitGroups = 2;                             // groups of 16 tokens to a warp's step
 constexpr int kUnitTokens = kUnitGroups * kGroupTokens;
 constexpr int kCombineThreads = 128;
+// What the end of a segment costs a CTA, in units: its warps wait for the last of them and join their parts.  Counted into the
+// list that is cut into ranges, or the CTAs among short contexts end last (64 requests of up to 8191 tokens: 128 us without).
+constexpr int kSegmentUnits = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ColumnParams {
@@ -253,11 +256,11 @@ __device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t 
 }
 
 __device__ __forceinline__ long long request_work(const ColumnParams &p, const Request &q) {
-  return static_cast<long long>(q.units) * q.column_groups * static_cast<long long>(p.call.cache.kv_heads);
+  return q.units == 0 ? 0 : static_cast<long long>(q.units + kSegmentUnits) * q.column_groups * static_cast<long long>(p.call.cache.kv_heads);
 }
 
 // A segment (kv head and column group of a request) of the list of all units: requests, then kv heads, then column groups,
-// then units.  Its ends count from the CTA's first unit; one that lies beyond 31 bits is as good as that.
+// then units and behind them kSegmentUnits places without work.  Its ends count from the CTA's first place.
 struct Cursor {
   uint32_t r;
   Request q;
@@ -273,7 +276,7 @@ struct Cursor {
           q = load_request(p, ++r, group_rows);
         while (q.units == 0);
       }
-      end = begin + q.units;
+      end = begin + q.units + kSegmentUnits;
     }
   }
 };
@@ -317,9 +320,10 @@ __device__ __forceinline__ long long find_start(const ColumnParams &p, int group
           break;
         before += w;
       }
-      c.segment = static_cast<int32_t>((u - before) / c.q.units);
-      c.begin = static_cast<int32_t>(before + static_cast<long long>(c.segment) * c.q.units - u);
-      c.end = c.begin + c.q.units;
+      const int32_t length = c.q.units + kSegmentUnits;
+      c.segment = static_cast<int32_t>((u - before) / length);
+      c.begin = static_cast<int32_t>(before + static_cast<long long>(c.segment) * length - u);
+      c.end = c.begin + length;
       *out = c;
     }
   }
@@ -392,9 +396,14 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
   size_t place = 0;
   auto fetch_page = [&]() {
     page = -1;
-    if (next >= units)
-      return;
-    ahead.seek(p, next, kRows);
+    for (;;) {  // (places without work are passed over, here and below)
+      if (next >= units)
+        return;
+      ahead.seek(p, next, kRows);
+      if (next - ahead.begin < ahead.q.units)
+        break;
+      next += (ahead.end - next + kWarps - 1) / kWarps * kWarps;
+    }
     if (lane < kUnitGroups) {
       const uint32_t group = static_cast<uint32_t>(ahead.q.first_unit + (next - ahead.begin)) * kUnitGroups + lane;
       if (static_cast<int32_t>(group) * kGroupTokens < ahead.q.len) {
@@ -484,14 +493,24 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
 
   Cursor at = start;
   int32_t u = warp;
+  bool rows_here = false;
+  if (threadIdx.x == 0)
+    ranges[blockIdx.x].valid = 0;
   for (int32_t from = 0; from < units;) {
     at.seek(p, from, kRows);
-    const int32_t seg_begin = at.begin, seg_end = at.end, to = seg_end < units ? seg_end : units;
+    const int32_t seg_begin = at.begin, seg_end = at.begin + at.q.units, to = seg_end < units ? seg_end : units;
+    if (seg_end <= from) {
+      from = at.end;
+      continue;
+    }
+    while (u < from)
+      u += kWarps;
     const int32_t head = at.segment / at.q.column_groups, column_group = at.segment - head * at.q.column_groups;
     const int32_t pair0 = column_group * kRows, pairs = min(kRows, at.q.rows * static_cast<int32_t>(p.group) - pair0);
 
-    if (from == 0)
+    if (!rows_here)
       load_rows(at);
+    rows_here = true;
     place_rows(at);  // (no warp is still in the products of the segment before)
     __syncthreads();
     float scale[NT][kMine];
@@ -733,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
 
     // ---- the warps' parts of the segment become one
     Cursor after = at;
-    if (to < units) {
-      after.seek(p, to, kRows);
+    if (at.end < units) {
+      after.seek(p, at.end, kRows);
       load_rows(after);
     }
 #pragma unroll
@@ -813,26 +832,24 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       if (j + 1 < NT)
         __syncthreads();
     }
-    if (threadIdx.x == 0 && to == units) {
+    if (threadIdx.x == 0 && !first && seg_end > units) {  // the CTA that holds the segment's last unit
+      const long long end = u0 + seg_end;
+      int last = static_cast<int>((end - 1) * ctas / work);
+      while (last + 1 < ctas && cta_begin(work, last + 1, ctas) < end)
+        ++last;
+      while (cta_begin(work, last, ctas) >= end)
+        --last;
       SplitRange range = {};
-      range.valid = !first && seg_end > units;
-      range.rows = at.q.rows;
-      range.first_row = at.q.first_row;
+      range.valid = 1;
       range.head = head;
       range.column_group = column_group;
-      if (range.valid) {  // the CTA that holds the segment's last unit
-        const long long end = u0 + seg_end;
-        int last = static_cast<int>((end - 1) * ctas / work);
-        while (last + 1 < ctas && cta_begin(work, last + 1, ctas) < end)
-          ++last;
-        while (cta_begin(work, last, ctas) >= end)
-          --last;
-        range.last_cta = last;
-      }
+      range.last_cta = last;
+      range.rows = at.q.rows;
+      range.first_row = at.q.first_row;
       ranges[blockIdx.x] = range;
     }
+    from = at.end;
     at = after;
-    from = to;
   }
 }
 
