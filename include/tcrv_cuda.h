@@ -456,8 +456,8 @@ typedef struct {
 int tcrv_cuda_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_stride, size_t k_head_stride,
                             const void *v, size_t v_row_stride, size_t v_head_stride, const int64_t *slots,
                             const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream);
-/* The inverse: k[row][head][d] and v (contiguous, d * q rounded to `type`) of the given slots; zeros
- * for a slot outside the cache. */
+/* The inverse: k[row][head][d] and v (contiguous, 16-byte aligned, d * q rounded to `type`) of the given
+ * slots; zeros for a slot outside the cache. */
 int tcrv_cuda_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *slots,
                            const tcrv_cuda_kv_cache *cache, tcrv_cuda_stream stream);
 

@@ -124,6 +124,7 @@ def test_attention_arguments(pkg):
         c = make(**changes)
         return L.tcrv_cuda_attention_q4_0_workspace_bytes(ctypes.addressof(c))
     assert size() > 0 and size(q=None, block_table=None, cache=cache(data=None)) == size()
+    assert size(rows=0) == 0 and size(max_new=1 << 20) == size(max_new=2)
     assert size(heads=5) == 0 and size(requests=0) == 0 and L.tcrv_cuda_attention_q4_0_workspace_bytes(None) == 0
 
 

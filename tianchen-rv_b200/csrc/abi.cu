@@ -757,7 +757,7 @@ size_t tcrv_cuda_attention_q4_0_workspace_bytes(const tcrv_cuda_attention_call *
     return 0;
   tcrv_cuda_attention_call c = *call;
   c.cache.pages = 0;  // (pointers do not matter here)
-  if (check_attention(c) != TCRV_CUDA_OK || c.requests == 0)
+  if (check_attention(c) != TCRV_CUDA_OK || c.requests == 0 || c.rows == 0)
     return 0;
   return attention_workspace_bytes(c);
 }

@@ -21,7 +21,7 @@ struct Shape {
   long long most_rows;
   // the prefill kernel
   bool prefill;
-  int row_blocks, splits;
+  int splits;
   size_t parts;
   size_t columns_bytes, prefill_offset, bytes;
 };
@@ -46,8 +46,7 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   s.prefill_offset = (s.columns_bytes + 255) / 256 * 256;
   s.bytes = s.columns_bytes;
   if (s.prefill) {
-    s.row_blocks = static_cast<int>((all + 2 * kTileRows - 1) / (2 * kTileRows));
-    const size_t items = static_cast<size_t>(s.row_blocks) * c.requests * c.cache.kv_heads;
+    const size_t items = (all + 2 * kTileRows - 1) / (2 * kTileRows) * c.requests * c.cache.kv_heads;
     // with fewer row blocks than half the SMs, each one's tokens are shared by several CTAs
     const size_t tiles = (c.width * c.cache.groups + kTileGroups - 1) / kTileGroups;
     size_t splits = items * 2 > static_cast<size_t>(sm_count()) ? 1 : sm_count() / items;
@@ -134,7 +133,6 @@ int launch_prefill(const tcrv_cuda_attention_call &c, const Shape &s, const Devi
   p.call.workspace = static_cast<uint8_t *>(c.workspace) + s.prefill_offset;
   p.group = static_cast<uint32_t>(c.heads / c.cache.kv_heads);
   p.min_rows = static_cast<int32_t>(kPrefillRows);
-  p.row_blocks = s.row_blocks;
   p.splits = s.splits;
   p.errors = errors;
   constexpr size_t smem = PrefillLayout<NB>::kBytes;

@@ -29,8 +29,9 @@ constexpr int kUnitGroups = 2;                             // groups of 16 token
 constexpr int kUnitTokens = kUnitGroups * kGroupTokens;
 constexpr int kCombineThreads = 128;
 // What the end of a segment costs a CTA, in units: its warps wait for the last of them and join their parts.  Counted into the
-// list that is cut into ranges, or the CTAs among short contexts end last (64 requests of up to 8191 tokens: 128 us without).
-constexpr int kSegmentUnits = 8;
+// list that is cut into ranges, or the CTAs among short contexts end last (64 requests of up to 8191 tokens: 128 us without, 118
+// with 8, 109 with 16 to 24, 113 with 40; 16 x 5 drafted tokens: 93, then 72, 76).
+constexpr int kSegmentUnits = 20;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ColumnParams {
@@ -347,7 +348,7 @@ __device__ __forceinline__ void write_row(const tcrv_cuda_attention_call &c, siz
 //
 // Bound by instructions, not by the 9/16 byte a value: a warp's unit of D = 128 and 8 rows takes about 880 (32 words unpacked
 // at 9 each, 32 products, the weights of each block, the soft-max, the copies' addresses), issued in 59 % of the cycles by 16
-// warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 89 us, 3.4 TB/s of cache; with (w & mask) | bits left to the compiler as two
+// warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 87 us, 3.5 TB/s of cache; with (w & mask) | bits left to the compiler as two
 // instructions, products that add to zeroed registers, and 64-bit cursors, 1100 instructions and 112 us.  Rows of several
 // tiles share a unit's unpacking (NT); their accumulators leave room for one CTA of 8 warps on an SM from 16 rows of 128 on.
 template <int NB, int NT, int MODE>

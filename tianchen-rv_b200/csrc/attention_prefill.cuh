@@ -43,7 +43,6 @@ struct PrefillParams {
   tcrv_cuda_attention_call call;
   uint32_t group;
   int32_t min_rows;      // requests with fewer rows (new tokens * group) are another kernel's
-  int32_t row_blocks;    // of a request at most
   int32_t splits;        // CTAs that share the tokens of one row block
   DeviceErrorWords errors;
 };
