@@ -87,7 +87,7 @@ struct RowTensor {
 };
 
 // One team of four lanes per (row, head, block), the key's block and the value's; teams run over blocks, then heads, then
-// rows, so a warp reads 8 adjacent blocks.  Bound by instructions, about 20 an element (8191 rows of 8 heads of 128, bf16:
+// rows, so a warp reads 8 adjacent blocks.  Bound by instructions, about 24 an element (8191 rows of 8 heads of 128, bf16:
 // 35 us with eight lanes to a block, which pay the item's arithmetic and the shuffles twice); a key's words of one token are
 // adjacent, a value's halfwords lie 4 bytes apart in 8 runs of 4 nb (they meet those of the group's other tokens in L2).
 // kBlocks: blocks to a row, 0 where only the call knows.
