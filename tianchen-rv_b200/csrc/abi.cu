@@ -741,7 +741,7 @@ int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream strea
   if (!call || call->page_tokens == 0)
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
   const tcrv_cuda_kv_plan_call &c = *call;
-  if (c.requests > 16384 || c.page_tokens > 65536 || c.rows > kManyRows || c.width > kManyRows / c.page_tokens ||
+  if (c.requests > kPlanRequests || c.page_tokens > 65536 || c.rows > kManyRows || c.width > kManyRows / c.page_tokens ||
       c.free_capacity > kManyRows)
     return TCRV_CUDA_ERR_UNSUPPORTED;
   if (!c.free_count || !c.first_rows || !c.info || (c.free_capacity != 0 && !c.free_pages) ||

@@ -2,6 +2,8 @@
 // quantises new rows into their slots, and the reader that gives slots back as numbers.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "kv_layout.cuh"
 #include "launchers.h"
 
@@ -238,6 +240,7 @@ int load_rows(void *k, void *v, size_t rows, const int64_t *slots, const tcrv_cu
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;           // one cluster of the portable size
 constexpr uint32_t kPlanAlone = 2048;  // rows and requests up to which one CTA does the step
+constexpr size_t kPlanSmem = (3 * kPlanRequests + 2) * sizeof(int32_t);  // of the largest call
 
 struct PlanSums {
   long long rows, pages;
@@ -416,8 +419,17 @@ int launch_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *
 
 int launch_kv_plan(const tcrv_cuda_kv_plan_call &call, cudaStream_t stream) {
   const size_t smem = (3 * call.requests + 2) * sizeof(int32_t);
-  if (smem > 48 * 1024)
-    TCRV_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  // The limit without asking counts the kernel's static shared memory too, and an attribute is the process's: what the largest
+  // call needs is asked for once on each device, before its first launch, and never taken back.
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  TCRV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64)
+    return TCRV_CUDA_ERR_UNSUPPORTED;
+  if (!done[dev]) {
+    TCRV_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPlanSmem)));
+    done[dev] = true;
+  }
   const bool alone = call.requests <= kPlanAlone && call.rows <= kPlanAlone;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(alone ? 1 : kPlanCtas);

@@ -53,6 +53,7 @@ int launch_kv_store_q4_0(int type, size_t rows, const void *k, size_t k_row_stri
                          cudaStream_t stream);
 int launch_kv_load_q4_0(int type, size_t rows, void *k, void *v, const int64_t *slots, const tcrv_cuda_kv_cache &cache,
                         cudaStream_t stream);
+constexpr size_t kPlanRequests = 16384;  // the most that a plan takes
 int launch_kv_plan(const tcrv_cuda_kv_plan_call &call, cudaStream_t stream);
 size_t attention_workspace_bytes(const tcrv_cuda_attention_call &call);
 int launch_attention_q4_0(const tcrv_cuda_attention_call &call, cudaStream_t stream);
