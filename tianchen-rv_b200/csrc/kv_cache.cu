@@ -68,8 +68,8 @@ __device__ __forceinline__ uint32_t quantise_team(const float (&v)[8], float *sc
   uint32_t bytes = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int q = static_cast<int>(__fadd_rn(__fmul_rn(v[j], id), 8.5f));  // (at least 0: |x / d| <= 8, and 0 for NaN)
-    bytes |= static_cast<uint32_t>(min(15, q)) << (8 * (j & 3) + (j & 4));
+    const int q = static_cast<int>(__fadd_rn(__fmul_rn(v[j], id), 8.5f));  // (0 for NaN; far outside 0..15 where |d| < 2^-128, whose reciprocal is infinite)
+    bytes |= static_cast<uint32_t>(max(0, min(15, q))) << (8 * (j & 3) + (j & 4));
   }
   *scale = d;
   return bytes;
