@@ -489,10 +489,10 @@ typedef struct {
 int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream stream);
 
 /* out[row][head] = softmax(scale * q[row][head] . K) V over the cache.  Request r's rows are
- * first_rows[r] .. first_rows[r+1] - 1 (at most max_new of them; without first_rows: row r alone), the
- * last tokens of the kv_lens[r] that it has in the pages block_table[r * table_stride ..]; row i of n
- * sees the tokens up to its own position kv_lens[r] - n + i and, if window > 0, only the last `window`
- * of those.  heads is a multiple of kv_heads, query heads h * (heads / kv_heads) .. share kv head h.
+ * first_rows[r] .. first_rows[r+1] - 1 (without first_rows: row r alone), the last tokens of the
+ * kv_lens[r] that it has in the pages block_table[r * table_stride ..]; row i of n sees the tokens up to
+ * its own position kv_lens[r] - n + i and, if window > 0, only the last `window` of those.  Rows from
+ * max_new on and rows behind `rows` are left out; the others keep their positions.  heads is a multiple of kv_heads, query heads h * (heads / kv_heads) .. share kv head h.
  * A row that sees nothing gets zeros and lse = -inf; rows outside every request are left as they were.
  * Tokens behind `width` pages and tokens in pages outside the cache count as unseen.  `lse` (may be
  * null) gets the natural logarithm of each row's soft-max sum, [row][head].  Strides count elements,

@@ -655,9 +655,10 @@ def attention_q4_0(q, cache, block_table, kv_lens, first_rows=None, max_new: int
     """softmax(scale * q K^T) V of each query row over its request's pages.
 
     q: (rows, heads, dim) float32, float16 or bfloat16, heads a multiple of the cache's; dim 64, 96,
-    128, 192 or 256.  Request r has the rows first_rows[r] .. first_rows[r + 1] - 1 (at most max_new; one
-    row each without first_rows), the last tokens of the kv_lens[r] that block_table[r] holds; a row sees
-    the tokens up to its own, with `window` only the last `window` of them.  scale: 1 / sqrt(dim).
+    128, 192 or 256.  Request r has the rows first_rows[r] .. first_rows[r + 1] - 1 (one row each without
+    first_rows), the last tokens of the kv_lens[r] that block_table[r] holds; a row sees the tokens up to
+    its own, with `window` only the last `window` of them.  Rows from max_new on are left out, the others
+    keep their positions.  scale: 1 / sqrt(dim).
     A row that sees nothing gives zeros (lse -inf); rows outside every request are left as they were.
     Returns out, or (out, lse) with lse (rows, heads) float32, the natural logarithm of the row's
     soft-max sum.  `workspace`: a uint8 tensor to use instead of a new one; calls that may overlap on the

@@ -218,9 +218,10 @@ __device__ __forceinline__ float scale_of(const uint32_t (&w)[N], int b) {
   return (b & 1) ? __high2float(h) : __low2float(h);
 }
 
-// What a call asks of one request.
+// What a call asks of one request.  `before` is the position of its first row: it counts all the rows that the request has, also
+// those that the call leaves out.
 struct Request {
-  int32_t rows, first_row, len, first_unit, units, column_groups;
+  int32_t rows, first_row, len, before, first_unit, units, column_groups;
 };
 
 __device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &c, uint32_t group, uint32_t r, int group_rows) {
@@ -228,6 +229,7 @@ __device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &
   long long first = c.first_rows ? c.first_rows[r] : r, end = c.first_rows ? c.first_rows[r + 1] : r + 1ll;
   if (first < 0)
     first = end = 0;
+  const long long all = end - first;
   if (end > static_cast<long long>(c.rows))
     end = static_cast<long long>(c.rows);
   long long rows = end - first;
@@ -238,8 +240,9 @@ __device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &
   q.rows = static_cast<int32_t>(rows);
   q.first_row = static_cast<int32_t>(first);
   q.len = static_cast<int32_t>(len);
+  q.before = static_cast<int32_t>(len - all);
   // the first row sees least far back
-  long long low = c.window ? len - rows + 1 - static_cast<long long>(c.window) : 0;
+  long long low = c.window ? len - all + 1 - static_cast<long long>(c.window) : 0;
   low = low < 0 ? 0 : low;
   q.first_unit = static_cast<int32_t>(low / kUnitTokens);
   const int32_t units = static_cast<int32_t>((len + kUnitTokens - 1) / kUnitTokens) - q.first_unit;
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       }
       if (lane == 0) {
         row_scale[i] = c.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
-        row_position[i] = i < pairs ? of.q.len - of.q.rows + (pair0 + i) / static_cast<int32_t>(p.group) : -1;
+        row_position[i] = i < pairs ? of.q.before + (pair0 + i) / static_cast<int32_t>(p.group) : -1;
       }
     }
   };

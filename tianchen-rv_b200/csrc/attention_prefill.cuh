@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   const int32_t block = blocks - 1 - from_end, pair0 = block * 2 * kTileRows;
   const int tiles_q = rows - pair0 > kTileRows ? 2 : 1;
   const int32_t last_pair = min(rows, pair0 + 2 * kTileRows) - 1;
-  const int32_t before = q.len - q.rows;  // position of the request's first row
+  const int32_t before = q.before;  // position of the request's first row
   const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
   const int32_t see_to = before + last_pair / static_cast<int32_t>(p.group);  // the last row sees furthest
   const int32_t see_from = window ? max(0, before + pair0 / static_cast<int32_t>(p.group) - window + 1) : 0;
