@@ -39,3 +39,11 @@ def test_fewer_rows_than_a_request_has(cuda, pkg, kind, window, max_new):
 @pytest.mark.parametrize("window", [0, 20])
 def test_rows_behind_the_queries(cuda, pkg, kind, window):
     case(cuda, pkg, kind, [150, 150], [0, 2, 92], 52, 90, 4, 2, 64, window=window, seed=4)
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("window", [0, 30, 300])
+@pytest.mark.parametrize("new", [1, 6, 80])
+def test_contexts_longer_than_their_table(cuda, pkg, kind, window, new):
+    # tokens behind the table are unseen, and the rows still sit at the end of the length
+    case(cuda, pkg, kind, [100, 2 ** 31 - 1, 120], [0, new, new + 1, 2 * new + 1], 2 * new + 1, new, 4, 2, 64, window=window, width=6, seed=new)

@@ -218,8 +218,8 @@ __device__ __forceinline__ float scale_of(const uint32_t (&w)[N], int b) {
   return (b & 1) ? __high2float(h) : __low2float(h);
 }
 
-// What a call asks of one request.  `before` is the position of its first row: it counts all the rows that the request has, also
-// those that the call leaves out.
+// What a call asks of one request.  `len` counts the tokens that its table has pages for; `before`, the position of its first row,
+// goes by all the tokens and rows that the request has, also those that the table or the call leaves out.
 struct Request {
   int32_t rows, first_row, len, before, first_unit, units, column_groups;
 };
@@ -234,16 +234,16 @@ __device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &
     end = static_cast<long long>(c.rows);
   long long rows = end - first;
   rows = rows < 0 ? 0 : rows > static_cast<long long>(c.max_new) ? static_cast<long long>(c.max_new) : rows;
-  long long len = c.kv_lens[r];
-  const long long most = static_cast<long long>(c.width) * c.cache.groups * kGroupTokens;
-  len = len < 0 ? 0 : len > most ? most : len;
+  const long long kv_len = c.kv_lens[r] < 0 ? 0 : c.kv_lens[r];
+  const long long most = static_cast<long long>(c.width) * c.cache.groups * kGroupTokens;  // a whole number of groups
+  const long long len = kv_len > most ? most : kv_len;
   q.rows = static_cast<int32_t>(rows);
   q.first_row = static_cast<int32_t>(first);
   q.len = static_cast<int32_t>(len);
-  q.before = static_cast<int32_t>(len - all);
+  q.before = static_cast<int32_t>(kv_len - all);
   // the first row sees least far back
-  long long low = c.window ? len - all + 1 - static_cast<long long>(c.window) : 0;
-  low = low < 0 ? 0 : low;
+  long long low = c.window ? kv_len - all + 1 - static_cast<long long>(c.window) : 0;
+  low = low < 0 ? 0 : low > len ? len : low;
   q.first_unit = static_cast<int32_t>(low / kUnitTokens);
   const int32_t units = static_cast<int32_t>((len + kUnitTokens - 1) / kUnitTokens) - q.first_unit;
   q.units = rows == 0 ? 0 : units < 1 ? 1 : units;  // (a request that sees nothing still writes its zeros)

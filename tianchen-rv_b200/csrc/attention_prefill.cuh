@@ -181,9 +181,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   const int32_t last_pair = min(rows, pair0 + 2 * kTileRows) - 1;
   const int32_t before = q.before;  // position of the request's first row
   const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
-  const int32_t see_to = before + last_pair / static_cast<int32_t>(p.group);  // the last row sees furthest
+  const int32_t see_to = min(before + last_pair / static_cast<int32_t>(p.group), q.len - 1);  // the last row sees furthest
   const int32_t see_from = window ? max(0, before + pair0 / static_cast<int32_t>(p.group) - window + 1) : 0;
-  int32_t tile_begin = see_from / kTileTokens, tile_end = see_to < 0 ? tile_begin : see_to / kTileTokens + 1;
+  int32_t tile_begin = see_from / kTileTokens, tile_end = see_to < see_from ? tile_begin : see_to / kTileTokens + 1;
   if (p.splits > 1) {
     const int32_t n = tile_end - tile_begin, b = tile_begin;
     tile_begin = b + static_cast<int32_t>(static_cast<int64_t>(n) * part / p.splits);
