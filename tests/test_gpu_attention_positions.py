@@ -47,3 +47,37 @@ def test_rows_behind_the_queries(cuda, pkg, kind, window):
 def test_contexts_longer_than_their_table(cuda, pkg, kind, window, new):
     # tokens behind the table are unseen, and the rows still sit at the end of the length
     case(cuda, pkg, kind, [100, 2 ** 31 - 1, 120], [0, new, new + 1, 2 * new + 1], 2 * new + 1, new, 4, 2, 64, window=window, width=6, seed=new)
+
+
+@pytest.mark.parametrize("kind,new", [("float32", 1), ("float16", 33)])
+def test_windows_beyond_2_to_the_30(cuda, pkg, kind, new):
+    """A context of 2^30 + 100 tokens (one page of nearly 2^20 again and again) whose first token decides: a window that holds it, and
+    one that ends before it."""
+    groups = 65535
+    page_tokens = 16 * groups
+    n = (1 << 30) + 100
+    width = -(-n // page_tokens)
+    rng = np.random.default_rng(0)
+    two = np.zeros((2, 1, groups, 18 * 64), np.uint8)
+    plain = ref.random_cache(rng, 1, 1, 16, 64)[0, 0, 0]
+    plain[16 * 64:17 * 64] = 0  # keys of zero
+    two[0, 0, :] = two[1, 0, :] = plain
+    key, value, shift, kd, vd = ref.places(64)
+    first = two[1, 0, 0]
+    quants = np.full((2, 16, 64), 8, np.uint8)
+    quants[:, 0] = 15
+    scales = np.full((2, 16, 2), 1.0, np.float16)
+    first[:] = ref.encode(quants[:, None], scales[:, None])[0]
+    cache = cuda.from_numpy(two).cuda()
+    table = cuda.zeros(1, width, dtype=cuda.int32, device="cuda")
+    table[0, 0] = 1
+    i32 = lambda x: cuda.tensor(x, dtype=cuda.int32, device="cuda")  # noqa: E731
+    q = cuda.ones(new, 1, 64, dtype=getattr(cuda, kind), device="cuda")
+    def run(window):
+        return pkg.attention_q4_0(q, cache, table, i32([n]), first_rows=i32([0, new]), max_new=new, window=window, scale=1.0)
+    seen = run(n)  # a score of 448 against zeros: the first token's values
+    pkg.check_device_errors()
+    assert bool((seen == 7.0).all())
+    last = run(n - 1)  # the last row does not see it, the others do
+    pkg.check_device_errors()
+    assert bool((last[:-1] == 7.0).all()) and bool((last[-1].abs() < 2.5).all())  # (a mean of values of at most 8 * 0.3)

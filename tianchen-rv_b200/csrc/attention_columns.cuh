@@ -251,6 +251,12 @@ __device__ __forceinline__ Request load_request(const tcrv_cuda_attention_call &
   return q;
 }
 
+// Positions are at most 2^31 - 2 and, held at -1 where a row sees nothing, at least -1: a window of 2^31 - 1 hides no token, and a
+// position less a window fits 32 bits.
+__device__ __forceinline__ int32_t window_of(const tcrv_cuda_attention_call &c) {
+  return static_cast<int32_t>(c.window < 0x7fffffffu ? c.window : 0x7fffffffu);
+}
+
 // The same for the kernel of this file: requests with more rows than it is meant for have no units.
 __device__ __forceinline__ Request load_request(const ColumnParams &p, uint32_t r, int group_rows) {
   Request q = load_request(p.call, p.group, r, group_rows);
@@ -490,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       }
       if (lane == 0) {
         row_scale[i] = c.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
-        row_position[i] = i < pairs ? of.q.before + (pair0 + i) / static_cast<int32_t>(p.group) : -1;
+        row_position[i] = i < pairs ? max(-1, of.q.before + (pair0 + i) / static_cast<int32_t>(p.group)) : -1;
       }
     }
   };
@@ -528,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         position[j][i] = row_position[row];
       }
     // tokens that every row of the group sees (rows are in order of position)
-    const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
+    const int32_t window = window_of(c);
     const int32_t seen_to = row_position[0], seen_from = window ? row_position[pairs - 1] - window + 1 : 0;
 
     float m[NT][kMine], l[NT][kMine], o[2 * NB][NT][4];

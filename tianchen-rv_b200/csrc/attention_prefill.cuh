@@ -180,9 +180,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   const int tiles_q = rows - pair0 > kTileRows ? 2 : 1;
   const int32_t last_pair = min(rows, pair0 + 2 * kTileRows) - 1;
   const int32_t before = q.before;  // position of the request's first row
-  const int32_t window = static_cast<int32_t>(c.window < 0x40000000u ? c.window : 0x40000000u);
+  const int32_t window = window_of(c);
+  // the first token that the row at `position` sees, of those that there are
+  const auto sees_from = [&](int32_t position) { return window ? max(0, max(-1, position) - window + 1) : 0; };
   const int32_t see_to = min(before + last_pair / static_cast<int32_t>(p.group), q.len - 1);  // the last row sees furthest
-  const int32_t see_from = window ? max(0, before + pair0 / static_cast<int32_t>(p.group) - window + 1) : 0;
+  const int32_t see_from = sees_from(before + pair0 / static_cast<int32_t>(p.group));
   int32_t tile_begin = see_from / kTileTokens, tile_end = see_to < see_from ? tile_begin : see_to / kTileTokens + 1;
   if (p.splits > 1) {
     const int32_t n = tile_end - tile_begin, b = tile_begin;
@@ -325,14 +327,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const auto state_of = [&](int tile, int lift) {
       const int32_t pair = pair0 + tile * kTileRows + row;
       State st;
-      st.position = pair < rows ? before + pair / group : -1;
+      st.position = pair < rows ? max(-1, before + pair / group) : -1;
       // (a row that sees nothing has a maximum, so that it does not hold up its warp)
       st.m = st.position < 0 ? 0.0f : -INFINITY;
       st.l = 0.0f;
       st.scale = fabsf(c.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - lift) << 23);
       const int32_t first = pair0 + tile * kTileRows;
-      st.from = window ? before + (min(rows, first + kTileRows) - 1) / group - window + 1 : 0;
-      st.to = before + first / group - (kTileTokens - 1);
+      st.from = sees_from(before + (min(rows, first + kTileRows) - 1) / group);
+      st.to = max(-1, before + first / group) - (kTileTokens - 1);
       return st;
     };
     State mine = state_of(0, static_cast<int8_t>(lifts)), other = state_of(1, static_cast<int8_t>(lifts >> 8));
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       const uint64_t group_flags = *reinterpret_cast<volatile uint64_t *>(smem + L::kFlags + slot * kTileGroups);
       const bool whole = group_flags == 0x0101010101010101ull && token0 >= mine.from && token0 <= mine.to;
       // columns that this row sees
-      const int32_t upper = mine.position - token0 - half * 64, lower = window ? upper - window + 1 : 0;
+      const int32_t upper = mine.position - token0 - half * 64, lower = window && window <= upper ? upper - window + 1 : 0;
       if (!whole) {  // scores in powers of two, unseen ones -infinity; the weights' scale is 1 then
         tmem_ld_wait();
 #pragma unroll
