@@ -1,0 +1,111 @@
+"""Attention over the paged Q4_0 cache: small values, values of many magnitudes side by side, values that are no numbers."""
+import numpy as np
+import pytest
+
+import attention_rms as rms
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = ["float16", "bfloat16"]
+
+
+def tensor(torch, x, kind):
+    t = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(getattr(torch, kind))
+    return t.cuda(), t.double().numpy()
+
+
+def ints(torch, x):
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device="cuda")
+
+
+def build(rng, lens, kv_heads, page_tokens, dim, keys, values):
+    """(cache, table) whose key and value scales are keys(r, shape) and values(r, shape) of request r, shape (kv_heads, tokens, dim / 32); any quants."""
+    table, pages = ref.tables(rng, lens, page_tokens)
+    lead = (pages, kv_heads, page_tokens // 16)
+    quants = rng.integers(0, 16, (2,) + lead + (16, dim), dtype=np.uint8)
+    scales = np.zeros((2,) + lead + (16, dim // 32))
+    for r, n in enumerate(lens):
+        held = -(-n // page_tokens)
+        for part, of in enumerate((keys, values)):
+            s = of(r, (kv_heads, held * page_tokens, dim // 32)).reshape(kv_heads, held, page_tokens // 16, 16, dim // 32)
+            scales[part][table[r, :held]] = s.transpose(1, 0, 2, 3, 4)
+    return ref.encode(quants, scales.astype(np.float16)), table
+
+
+def call(torch, pkg, q, cache, table, lens, first, **k):
+    return pkg.attention_q4_0(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table.astype(np.int32)).cuda(), ints(torch, lens),
+                              first_rows=ints(torch, first), max_new=int(np.diff(first).max()), with_lse=True, **k)
+
+
+def ordinary(rng):
+    return lambda r, shape: rng.uniform(0.02, 0.3, shape) * rng.choice((-1.0, 1.0), shape)
+
+
+def few_rows(torch, pkg, kind, lens, new, heads, kv_heads, dim, values, seed=0, sink=None, page_tokens=32, prompt=False):
+    rng = np.random.default_rng(seed)
+    cache, table = build(rng, lens, kv_heads, page_tokens, dim, ordinary(rng), values(rng))
+    first = np.concatenate(([0], np.cumsum(new)))
+    x = rng.standard_normal((first[-1], heads, dim))
+    if sink is not None:  # one token `sink` above the rest: its key is along every query of its head
+        toward = rng.standard_normal((kv_heads, dim))
+        x = np.repeat(toward, heads // kv_heads, 0)[None] + 0.05 * x
+        key, _, shift, kd, _ = ref.places(dim)
+        quants, size = np.clip(np.rint(toward / 0.4) + 8, 0, 15).astype(np.uint8), 0.4
+        size = sink / (dim ** -0.5 * ((quants - 8.0) * toward).sum(-1))  # its score
+        for r in range(len(lens)):
+            for h in range(kv_heads):
+                group, token = cache[table[r, 0], h, 0], 5
+                for d in range(dim):
+                    group[key[token, d]] = group[key[token, d]] & (0xf0 >> shift[token, d]) | quants[h, d] << shift[token, d]
+                group[np.add.outer(kd[token], np.arange(2))] = np.array([size[h]], np.float16).view(np.uint8)
+    q, q64 = tensor(torch, x, kind)
+    got, lse = call(torch, pkg, q, cache, table, lens, first)
+    pkg.check_device_errors()
+    d = rms.definition(q64, cache, table, lens, first, dim ** -0.5)
+    rms.check(got, lse, d, kind, prompt)
+
+
+@pytest.mark.parametrize("kind", HALF + ["float32"])
+@pytest.mark.parametrize("spread", [1.0, 1e-2, 1e-3, 1e-4, 1e-5])
+def test_small_values_of_few_rows(cuda, pkg, kind, spread):
+    few_rows(cuda, pkg, kind, [2900, 70], [1, 1], 8, 2, 128, lambda rng: lambda r, s: ordinary(rng)(r, s) * spread, seed=1)
+
+
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("dim,heads,new", [(64, 4, [5, 3]), (96, 4, [1, 2]), (128, 12, [5, 1]), (192, 4, [1, 5]), (256, 2, [9, 2])])
+def test_small_values_of_every_head_size(cuda, pkg, kind, dim, heads, new):
+    few_rows(cuda, pkg, kind, [1500, 300], new, heads, 1, dim, lambda rng: lambda r, s: ordinary(rng)(r, s) * 1e-4, seed=dim)
+
+
+@pytest.mark.parametrize("kind", HALF + ["float32"])
+@pytest.mark.parametrize("spread", [1.0, 1e-1, 1e-2, 1e-3])
+def test_one_token_above_the_rest(cuda, pkg, kind, spread):
+    # the heavy token's values are a hundredth of the others'
+    def values(rng):
+        def of(r, shape):
+            s = ordinary(rng)(r, shape) * spread
+            s[:, 5] *= 0.01
+            return s
+        return of
+    few_rows(cuda, pkg, kind, [2900, 700], [1, 1], 8, 2, 128, values, seed=2, sink=8.0)
+
+
+@pytest.mark.parametrize("kind", HALF + ["float32"])
+def test_values_that_grow_along_the_context(cuda, pkg, kind):
+    # the largest scale seen moves again and again, up to fp16's largest
+    few_rows(cuda, pkg, kind, [1400], [1], 4, 1, 128,
+             lambda rng: lambda r, s: ordinary(rng)(r, s) * np.exp(np.linspace(np.log(2e-6), np.log(2e5), s[1]))[None, :, None], seed=3)
+
+
+@pytest.mark.parametrize("kind", HALF + ["float32"])
+def test_values_of_zero(cuda, pkg, kind):
+    # no scale at all in the first request, one token's in the second
+    def values(rng):
+        def of(r, shape):
+            s = np.zeros(shape)
+            if r:
+                s[:, 33] = 1e-3
+            return s
+        return of
+    few_rows(cuda, pkg, kind, [100, 100], [1, 2], 4, 2, 64, values, seed=4)

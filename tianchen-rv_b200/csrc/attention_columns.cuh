@@ -9,11 +9,13 @@
 // Numbers.  A cached value is d * (n - 8).  Its integer part is exact in fp16 and the products with it are
 // summed in f32; the scales stay outside: the key's multiplies the f32 sum over its block, the value's
 // multiplies the soft-max weight, one operand per block.  What is rounded is the query row (scaled by a
-// power of two so that its largest element lies in [2^14, 2^15)) and the weight times the value's scale:
-//   fp16 and bf16 calls: both to one fp16 term, 2^-12 relative (a 16-bit query is exact);
+// power of two so that its largest element lies in [2^14, 2^15)) and the weight times the value's scale
+// (lifted by a power of two that brings the largest scale seen so far into [2^14, 2^15)):
+//   fp16 and bf16 calls: both to one fp16 term, half a step of 2^-11 (a 16-bit query is exact);
 //   f32 calls: both to two fp16 terms, 2^-22 relative, with a product each into the same sums, or up to 4
-//   rows with a column each (777 tokens, 4 rows: 19 us against 15).  The value
-//   scales are lifted by a power of two that follows the largest one seen, like the running maximum.
+//   rows with a column each (777 tokens, 4 rows: 19 us against 15).
+// A weight times its scale leaves fp16's normal range below 2^-28 of the largest scale: what it then loses is at most 2^-39 of that
+// scale.  (Without a lift values of 1e-4 lost a percent, and those beside a token e^8 above them more.)
 // Maximum, sum and accumulators are f32.
 #pragma once
 
@@ -95,6 +97,11 @@ __device__ __forceinline__ void mma16816_zero(float (&c)[4], const uint32_t (&a)
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// What lifts scales below `ceiling`, a power of two in 2^-24 .. 2^16, below 2^15: 2^15 / ceiling, exactly.
+__device__ __forceinline__ float lift_of(float ceiling) {
+  return __uint_as_float(((127u + 15u + 127u) << 23) - __float_as_uint(ceiling));
 }
 
 // 8 x 8 transpose of 16-bit elements held two to a lane.
@@ -538,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
     const int32_t seen_to = row_position[0], seen_from = window ? row_position[pairs - 1] - window + 1 : 0;
 
     float m[NT][kMine], l[NT][kMine], o[2 * NB][NT][4];
-    int lifted = -100;  // exponent of the largest value scale so far; the accumulators hold O * 2^(14 - lifted)
+    float ceiling = 0x1p-24f;  // the power of two above the largest value scale so far; the accumulators hold O * lift_of(ceiling)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -566,6 +573,16 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
       const uint8_t *unit = ring + stage * L::kUnitBytes;
       const uint32_t there = flags[stage];
       const int32_t token0 = (at.q.first_unit + (u - seg_begin)) * kUnitTokens;
+
+      // ---- the largest value scale, a word or two to a lane (early, for the warp's maximum takes its time; NaN counts as nothing)
+      __half2 most = __float2half2_rn(0.0f);
+#pragma unroll
+      for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+        for (int i = 0; i < 8 * NB; i += 32)
+          if (8 * NB % 32 == 0 || i + lane < 8 * NB)
+            most = __hmax2(most, __habs2(*reinterpret_cast<const __half2 *>(unit + gr * kGroupBytes + 544 * NB + 4 * (i + lane))));
+      uint32_t top_scale = __reduce_max_sync(0xffffffffu, __half_as_ushort(__hmax(__low2half(most), __high2half(most))));
 
       // ---- S^T = K q^T
       float s[kUnitGroups][NT][4];
@@ -660,39 +677,39 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
               vd[gr][h][b] = there_is ? vd[gr][h][b] : 0u;
           }
         }
-      float lift = 1.0f, relift = 1.0f;
-      if constexpr (MODE != kOneTerm) {
-        const auto largest = [&](bool finite_only) {
-          __half2 most = __float2half2_rn(0.0f);
+      // ---- the lift follows the largest of them that a row may see; beside infinities and NaNs it goes by the others
+      if (!whole || top_scale >= 0x7c00u) {
+        uint32_t top = 0;
 #pragma unroll
-          for (int gr = 0; gr < kUnitGroups; ++gr)
+        for (int gr = 0; gr < kUnitGroups; ++gr)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int b = 0; b < (NB + 1) / 2; ++b) {
-                uint32_t d = vd[gr][h][b] & 0x7fff7fffu;
-                if (finite_only)
-                  d &= ((d & 0x7c00u) == 0x7c00u ? 0xffff0000u : ~0u) & ((d & 0x7c000000u) == 0x7c000000u ? 0xffffu : ~0u);
-                most = __hmax2(most, bits_half2(d));
-              }
-          float top = fmaxf(__low2float(most), __high2float(most));
-#pragma unroll
-          for (int off = 4; off <= 16; off <<= 1)
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          return top;
-        };
-        float top = largest(false);
-        if (top == INFINITY)  // (of a token that some rows may not see: their lift goes by the others)
-          top = largest(true);
-        // exponent of an fp16 number, -100 for zero
-        const int e = top > 0.0f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 : -100;
-        if (e > lifted) {
-          relift = exp2f(static_cast<float>(lifted - e));
-          lifted = e;
-          moved = true;
-        }
-        lift = lifted > -100 ? exp2f(static_cast<float>(14 - lifted)) : 1.0f;
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t d = (b & 1 ? vd[gr][h][b / 2] >> 16 : vd[gr][h][b / 2]) & 0x7fffu;
+              top = max(top, d < 0x7c00u ? d : 0u);
+            }
+        top_scale = __reduce_max_sync(0xffffffffu, top);
       }
+      const float top = half_bits_to_float(top_scale);
+      float relift = 1.0f;
+      if (top >= ceiling) {
+        const uint32_t now = (__float_as_uint(top) & 0x7f800000u) + 0x00800000u;  // the next power of two
+        relift = __uint_as_float(0x3f800000u + __float_as_uint(ceiling) - now);
+        ceiling = __uint_as_float(now);
+        moved = true;
+      }
+      const float lift = lift_of(ceiling);
+#pragma unroll
+      for (int gr = 0; gr < kUnitGroups; ++gr)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 x = mul2(make_float2(pr[gr][j][h][0], pr[gr][j][h][kMine - 1]), make_float2(lift, lift));
+            pr[gr][j][h][0] = x.x;
+            pr[gr][j][h][kMine - 1] = x.y;
+          }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i)
@@ -723,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
             uint32_t bits[kProducts][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float d = MODE == kOneTerm ? scale_of(vd[gr][h], b) : scale_of(vd[gr][h], b) * lift;
+              const float d = scale_of(vd[gr][h], b);
               if constexpr (MODE == kPairs) {
                 float v = pr[gr][j][h][0] * d;
                 if (!whole)
@@ -796,8 +813,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         f[i] = m[j][i] == -INFINITY ? 0.0f : exp2_fast(m[j][i] - top);
         if (g == 0)
           stats[(warp * kRows + row) * 2 + 1] = l[j][i] * f[i];
-        if constexpr (MODE != kOneTerm)
-          f[i] *= lifted > -100 ? exp2f(static_cast<float>(lifted - 14)) : 1.0f;
+        f[i] *= ceiling * 0x1p-15f;
       }
       float *mine = sums + warp * kTileRows * kDim;
 #pragma unroll
