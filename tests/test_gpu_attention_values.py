@@ -109,3 +109,20 @@ def test_values_of_zero(cuda, pkg, kind):
             return s
         return of
     few_rows(cuda, pkg, kind, [100, 100], [1, 2], 4, 2, 64, values, seed=4)
+
+
+@pytest.mark.parametrize("new", [1, 4, 30])
+def test_values_that_no_row_sees_do_not_matter(cuda, pkg, new):
+    """f32: tokens before the window with the largest scales there are, among values of 1e-5."""
+    rng = np.random.default_rng(new)
+    n, window = 213, 40
+    first = n - new - window + 1  # the first token that a row sees
+    def values(r, shape):
+        s = rng.uniform(2e-6, 1e-5, shape)
+        s[:, :first] = 6e4
+        return s
+    cache, table = build(rng, [n], 1, 16, 64, ordinary(rng), values)
+    q, q64 = tensor(cuda, rng.standard_normal((new, 2, 64)), "float32")
+    got, lse = call(cuda, pkg, q, cache, table, [n], [0, new], window=window)
+    d = rms.definition(q64, cache, table, [n], [0, new], 64 ** -0.5, window)
+    rms.check(got, lse, d, "float32")

@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
           l[j][i] = fmaf(l[j][i], alpha[j][i], sum);
         }
 
-      // ---- value scales of this lane's tokens; those of unseen tokens may be anything and count as zero
+      // ---- value scales of this lane's tokens; those of tokens that no row sees may be anything and count as zero
       uint32_t vd[kUnitGroups][2][(NB + 1) / 2];
 #pragma unroll
       for (int gr = 0; gr < kUnitGroups; ++gr)
@@ -671,7 +671,8 @@ __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(
         for (int h = 0; h < 2; ++h) {
           load_scales<NB>(vd[gr][h], unit + gr * kGroupBytes + 544 * NB + (g + 8 * h) * NB * 2);
           if (!whole) {
-            const bool there_is = ((there >> gr) & 1u) && token0 + gr * kGroupTokens + h * 8 + g < at.q.len;
+            const int32_t token = token0 + gr * kGroupTokens + h * 8 + g;
+            const bool there_is = ((there >> gr) & 1u) && token <= row_position[pairs - 1] && !(window && token <= row_position[0] - window);
 #pragma unroll
             for (int b = 0; b < (NB + 1) / 2; ++b)
               vd[gr][h][b] = there_is ? vd[gr][h][b] : 0u;
