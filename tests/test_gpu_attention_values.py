@@ -111,6 +111,47 @@ def test_values_of_zero(cuda, pkg, kind):
     few_rows(cuda, pkg, kind, [100, 100], [1, 2], 4, 2, 64, values, seed=4)
 
 
+# prompts: rows enough for the kernel whose operands are fp16
+
+
+def prompt_case(torch, pkg, kind, n, new, heads, kv_heads, dim, keys, values, seed, window=0, std=1.0):
+    """(definition, got, lse) of one request."""
+    rng = np.random.default_rng(seed)
+    cache, table = build(rng, [n], kv_heads, 32, dim, keys(rng), values(rng))
+    q, q64 = tensor(torch, rng.standard_normal((new, heads, dim)) * std, kind)
+    got, lse = call(torch, pkg, q, cache, table, [n], [0, new], window=window)
+    pkg.check_device_errors()
+    return rms.definition(q64, cache, table, [n], [0, new], dim ** -0.5, window), got, lse
+
+
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("n,new,dim", [(700, 400, 128), (1500, 33, 128), (300, 300, 64), (4000, 40, 64)])
+def test_prompts_on_average(cuda, pkg, kind, n, new, dim):
+    d, got, lse = prompt_case(cuda, pkg, kind, n, new, 4, 2, dim, ordinary, ordinary, seed=n)
+    rms.check(got, lse, d, kind, True)
+
+
+@pytest.mark.parametrize("n,new,kind", [(300, 250, "bfloat16"), (300, 250, "float16"), (2500, 40, "bfloat16"), (300, 3, "bfloat16"), (300, 3, "float32")])
+def test_a_value_scale_that_is_no_number_reaches_its_block_only(cuda, pkg, n, new, kind):
+    """Rows that see the token have no numbers in the 32 elements of the block; everything else, the soft-max sum too, is as without it."""
+    rng = np.random.default_rng(n)
+    cache, table = build(rng, [n], 2, 16, 128, ordinary(rng), ordinary(rng))
+    q, q64 = tensor(cuda, rng.standard_normal((new, 4, 128)), kind)
+    d = rms.definition(q64, cache, table, [n], [0, new], 128 ** -0.5)
+    _, _, _, _, vd = ref.places(128)
+    prompt = new * 2 > 32
+    for bits in (0x7c00, 0xfc00, 0x7e00):
+        for token, block in ((n - 20, 0), (60, 3), (n - 1, 2)):
+            spoiled = cache.copy()
+            spoiled[table[0, token // 16], 1, 0, vd[token % 16, block]] = bits & 255
+            spoiled[table[0, token // 16], 1, 0, vd[token % 16, block] + 1] = bits >> 8
+            got, lse = call(cuda, pkg, q, spoiled, table, [n], [0, new])
+            reached = np.zeros(got.shape, bool)
+            reached[max(0, token - (n - new)):, 2:, 32 * block:32 * block + 32] = True
+            assert not np.isfinite(got.float().cpu().numpy()[reached]).any()
+            rms.check(got, lse, d, kind, prompt, where=~reached)
+
+
 @pytest.mark.parametrize("new", [1, 4, 30])
 def test_values_that_no_row_sees_do_not_matter(cuda, pkg, new):
     """f32: tokens before the window with the largest scales there are, among values of 1e-5."""

@@ -63,8 +63,9 @@ struct PrefillLayout {
   static constexpr int kKey = kQuery + 2 * kKeyBytes;
   static constexpr int kValue = kKey + 2 * kKeyBytes;
   static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
-  static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group]: tokens with a value scale that is no number
-  static constexpr int kBars = kPoison + kSlots * kTileGroups * 2;
+  static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group][block]: tokens whose value scale is no number
+  static constexpr int kBadRows = kPoison + kSlots * kTileGroups * NB * 2;  // u8 [tile][half][row]: blocks of which it sees such a token
+  static constexpr int kBars = kBadRows + 2 * 2 * 128;
   static constexpr int kBarCount = 20;
   static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
   static constexpr int kTmem = kTops + 2 * 2 * 128 * 4;
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + L::kAbort);
   volatile uint8_t *flags = smem + L::kFlags;
   volatile uint16_t *poison = reinterpret_cast<volatile uint16_t *>(smem + L::kPoison);
+  volatile uint8_t *bad_rows = smem + L::kBadRows;
   const tcrv_cuda_attention_call &c = p.call;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -240,6 +242,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const int32_t group = static_cast<int32_t>(p.group);
     float *tops = reinterpret_cast<float *>(smem + L::kTops);
     int lifts = 0;  // powers of the queries of this thread's row in the two tiles, a byte each
+    bad_rows[half * 128 + row] = bad_rows[(2 + half) * 128 + row] = 0;
     {
       // ---- the query operand, tile `half`: 32 rows of it, in the key operand's order of elements, times a power of two that
       // lifts the largest element into [2^14, 2^15).  kDim / 8 lanes to a row, eight elements to a lane.
@@ -436,11 +439,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
             for (int i = 8 * h; i < 8 * h + 8; ++i)
               w[i] = half2_bits(__hmul2(bits_half2(w[i]), __float2half2_rn(16.0f)));
           }
-          if (flag & 8u) {  // a value that is no number: the rows that see its token are none either
-            const uint32_t bad = poison[slot * kTileGroups + 4 * half + h];
-            for (int i = 0; i < kGroupTokens; ++i)
-              if (((bad >> i) & 1u) && 16 * h + i <= upper && 16 * h + i >= lower)
-                mine.l = NAN;
+          if (flag & 8u) {  // values that are no numbers: nor are the elements of their block, of the rows that see their token
+            const int32_t first = max(lower - 16 * h, 0), last = min(upper - 16 * h, kGroupTokens - 1);
+            const uint32_t seen = first <= last ? (2u << last) - (1u << first) : 0u;
+            uint32_t blocks = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              blocks |= (poison[(slot * kTileGroups + 4 * half + h) * NB + b] & seen) ? 1u << b : 0u;
+            if (blocks)
+              bad_rows[(tile * 2 + half) * 128 + row] |= static_cast<uint8_t>(blocks);
           }
         }
       }
@@ -477,6 +484,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       float l = st.l;
       if (wait(kBarPair + (warp & 3), steps + 1 + tile))
         l = half == 0 ? l + exchange[128 + row] : exchange[row] + l;
+      const uint32_t bad = bad_rows[tile * 2 * 128 + row] | bad_rows[(tile * 2 + 1) * 128 + row];
       const int32_t pair = pair0 + tile * kTileRows + row, token = pair / group;
       const size_t q_head = static_cast<size_t>(head) * group + (pair - token * group);
       const size_t at = static_cast<size_t>(q.first_row + token) * c.out_row_stride + q_head * c.out_head_stride;
@@ -493,7 +501,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
 #pragma unroll
         for (int d = 0; d < 32; ++d) {
           const float v = __uint_as_float(o[(d >> 4) * 16 + (d & 1) * 8 + ((d & 15) >> 1)]);
-          y[d] = any ? v * factor : 0.0f;  // (without a product the columns hold anything)
+          y[d] = (bad >> b) & 1u ? NAN : any ? v * factor : 0.0f;  // (without a product the columns hold anything)
         }
         if (pair < rows) {
           if (part_sums != nullptr) {
@@ -614,7 +622,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       // which does no harm
       if (__any_sync(0xffffffffu, (some & 0x7000u) == 0x7000u || (some & 0x70000000u) == 0x70000000u)) {
         const __half2 sixteenth = __float2half2_rn(0.0625f);
-        uint32_t bad = 0;
+        uint32_t bad[NB] = {}, any_bad = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -623,20 +631,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             if ((pair[h][b] & 0x7c00u) == 0x7c00u) {
-              bad |= 1u << (2 * t + 8 * h);
+              bad[b] |= 1u << (2 * t + 8 * h);
               pair[h][b] &= 0xffff0000u;
             }
             if ((pair[h][b] & 0x7c000000u) == 0x7c000000u) {
-              bad |= 2u << (2 * t + 8 * h);
+              bad[b] |= 2u << (2 * t + 8 * h);
               pair[h][b] &= 0xffffu;
             }
             pair[h][b] = half2_bits(__hmul2(bits_half2(pair[h][b]), sixteenth));
           }
         }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        flag |= bad ? 14u : 6u;
-        if (lane == 0)
-          poison[slot * kTileGroups + w] = static_cast<uint16_t>(bad);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          bad[b] = __reduce_or_sync(0xffffffffu, bad[b]);
+          any_bad |= bad[b];
+          if (lane == 0)
+            poison[(slot * kTileGroups + w) * NB + b] = static_cast<uint16_t>(bad[b]);
+        }
+        flag |= any_bad ? 14u : 6u;
       }
       if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
         return false;
