@@ -131,6 +131,58 @@ def test_prompts_on_average(cuda, pkg, kind, n, new, dim):
     rms.check(got, lse, d, kind, True)
 
 
+SMALL = {"float16": (6.2e-5, 1e-4), "bfloat16": (1e-5, 2e-5)}  # (a scale below 2^-14 times a quant is a whole number of fp16's steps)
+
+
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("n,new", [(260, 200), (2100, 40)])
+def test_prompts_with_large_scales_beside_small_ones(cuda, pkg, kind, n, new):
+    """Block 0 of a value has scales of 0.13 and 2.1, block 1 of 1e-4 or less, in the same group of tokens."""
+    def values(rng):
+        def of(r, shape):
+            s = rng.uniform(*SMALL[kind], shape)
+            s[..., 0] = np.where(np.arange(shape[1]) % 2, 0.13, 2.1)
+            return s
+        return of
+    d, got, lse = prompt_case(cuda, pkg, kind, n, new, 8, 2, 64, ordinary, values, seed=n, window=8)
+    rms.check(got, lse, d, kind, True)
+    rms.check(got, None, d, kind, True, where=np.broadcast_to(np.arange(64) >= 32, got.shape))
+
+
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("part", ["keys", "values"])
+@pytest.mark.parametrize("n", [48, 2096])
+def test_prompts_before_a_token_that_leaves_fp16(cuda, pkg, kind, part, n):
+    """The last token has scales of 2^13 and more, so that its values leave fp16; rows before it see the small ones beside it as they are."""
+    def large(rng):
+        def of(r, shape):
+            s = rng.uniform(*SMALL[kind], shape)
+            s[:, n - 1] = rng.uniform(8192, 60000, shape[2])
+            return s
+        return of
+    keys, values = (large, ordinary) if part == "keys" else (ordinary, large)
+    d, got, lse = prompt_case(cuda, pkg, kind, n, 40, 8, 1, 64, keys, values, seed=n, window=8, std=1e4 if part == "keys" else 1.0)
+    near = np.zeros(got.shape, bool)
+    near[31:39] = True  # rows that see this group's tokens only, and not the last one
+    d["lse"][~near[..., 0]] = np.nan
+    rms.check(got, lse, d, kind, True, where=near)
+
+
+@pytest.mark.parametrize("kind", HALF)
+def test_prompts_with_tokens_that_leave_fp16(cuda, pkg, kind):
+    """Keys and values of 2^13 and more here and there, seen by all rows."""
+    def few(rng):
+        def of(r, shape):
+            s = ordinary(rng)(r, shape)
+            s[:, 7::50] = rng.uniform(8192, 60000, s[:, 7::50].shape)
+            return s
+        return of
+    d, got, lse = prompt_case(cuda, pkg, kind, 300, 60, 2, 1, 64, few, few, seed=9, std=2e-5)
+    if kind == "float16":
+        d["out"][np.abs(d["out"]).max(-1) > 6e4] = np.nan  # (a result that its type does not hold)
+    rms.check(got, lse, d, kind, True)
+
+
 @pytest.mark.parametrize("n,new,kind", [(300, 250, "bfloat16"), (300, 250, "float16"), (2500, 40, "bfloat16"), (300, 3, "bfloat16"), (300, 3, "float32")])
 def test_a_value_scale_that_is_no_number_reaches_its_block_only(cuda, pkg, n, new, kind):
     """Rows that see the token have no numbers in the 32 elements of the block; everything else, the soft-max sum too, is as without it."""

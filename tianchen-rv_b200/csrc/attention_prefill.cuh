@@ -15,7 +15,7 @@
 //
 // Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
 // scaled block by block without reading S and O once for every block of 32.  Query rows are fp16 after a power of two
-// (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A group with a scale so large that
+// (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A token with a scale so large that
 // its values leave fp16 is held at 1/16 and made good in S or in P.  The running maximum that P is relative to follows the
 // true one only when that has grown by more than 2^8: then O is rescaled, otherwise P just has values up to 2^8.
 #pragma once
@@ -64,7 +64,8 @@ struct PrefillLayout {
   static constexpr int kValue = kKey + 2 * kKeyBytes;
   static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
   static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group][block]: tokens whose value scale is no number
-  static constexpr int kBadRows = kPoison + kSlots * kTileGroups * NB * 2;  // u8 [tile][half][row]: blocks of which it sees such a token
+  static constexpr int kHeld = kPoison + kSlots * kTileGroups * NB * 2;     // u32 [slot][group]: tokens held at 1/16, keys, values << 16
+  static constexpr int kBadRows = kHeld + kSlots * kTileGroups * 4;         // u8 [tile][half][row]: blocks of which it sees such a token
   static constexpr int kBars = kBadRows + 2 * 2 * 128;
   static constexpr int kBarCount = 20;
   static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
@@ -159,6 +160,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + L::kAbort);
   volatile uint8_t *flags = smem + L::kFlags;
   volatile uint16_t *poison = reinterpret_cast<volatile uint16_t *>(smem + L::kPoison);
+  volatile uint32_t *held = reinterpret_cast<volatile uint32_t *>(smem + L::kHeld);
   volatile uint8_t *bad_rows = smem + L::kBadRows;
   const tcrv_cuda_attention_call &c = p.call;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -363,11 +365,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (4 * half + h)));
-          const float by = (flag & 2u) ? 16.0f * mine.scale : mine.scale;
+          if (flag & 2u) {  // keys held at 1/16
+            const uint32_t keys = held[slot * kTileGroups + 4 * half + h];
+#pragma unroll
+            for (int i = 0; i < kGroupTokens; ++i)
+              s[16 * h + i] = (keys >> i) & 1u ? __float_as_uint(16.0f * __uint_as_float(s[16 * h + i])) : s[16 * h + i];
+          }
           const int32_t to = (flag & 1u) ? upper : -1;
 #pragma unroll
           for (int i = 16 * h; i < 16 * h + 16; ++i)
-            s[i] = i <= to && i >= lower ? __float_as_uint(__uint_as_float(s[i]) * by) : 0xff800000u;
+            s[i] = i <= to && i >= lower ? __float_as_uint(__uint_as_float(s[i]) * mine.scale) : 0xff800000u;
         }
       }
       const float by = whole ? mine.scale : 1.0f;
@@ -435,9 +442,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         for (int h = 0; h < 4; ++h) {
           const uint32_t flag = static_cast<uint32_t>(group_flags >> (8 * (4 * half + h)));
           if (flag & 4u) {  // values held at 1/16
+            const uint32_t values = held[slot * kTileGroups + 4 * half + h] >> 16;
 #pragma unroll
-            for (int i = 8 * h; i < 8 * h + 8; ++i)
-              w[i] = half2_bits(__hmul2(bits_half2(w[i]), __float2half2_rn(16.0f)));
+            for (int i = 0; i < 8; ++i)
+              w[8 * h + i] = half2_bits(__hmul2(bits_half2(w[8 * h + i]), __floats2half2_rn((values >> (2 * i)) & 1u ? 16.0f : 1.0f, (values >> (2 * i)) & 2u ? 16.0f : 1.0f)));
           }
           if (flag & 8u) {  // values that are no numbers: nor are the elements of their block, of the rows that see their token
             const int32_t first = max(lower - 16 * h, 0), last = min(upper - 16 * h, kGroupTokens - 1);
@@ -618,18 +626,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
         }
       }
       uint32_t flag = now.there ? 1u : 0u;
-      // a scale of 2^13 or more (8 d may leave fp16), an infinity or a NaN has these three bits; so may several others together,
-      // which does no harm
+      // A scale of 2^13 or more (8 d may leave fp16), an infinity or a NaN has these three bits; so may several others together.  Then
+      // the tokens that have one are looked for and held at 1/16, which others of the group would not bear (below 2^-10 a sixteenth is
+      // not exact).
       if (__any_sync(0xffffffffu, (some & 0x7000u) == 0x7000u || (some & 0x70000000u) == 0x70000000u)) {
-        const __half2 sixteenth = __float2half2_rn(0.0625f);
-        uint32_t bad[NB] = {}, any_bad = 0;
+        uint32_t bad[NB] = {}, any_bad = 0, large = 0;  // large: keys' tokens, values' << 16
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int b = 0; b < NB / 2; ++b)
-            now.key_scale[h][b] = half2_bits(__hmul2(bits_half2(now.key_scale[h][b]), sixteenth));
-#pragma unroll
           for (int b = 0; b < NB; ++b) {
+            const uint32_t d = (b & 1) ? now.key_scale[h][b / 2] >> 16 : now.key_scale[h][b / 2];
+            large |= (d & 0x7000u) == 0x7000u ? 1u << (g + 8 * h) : 0u;
             if ((pair[h][b] & 0x7c00u) == 0x7c00u) {
               bad[b] |= 1u << (2 * t + 8 * h);
               pair[h][b] &= 0xffff0000u;
@@ -638,8 +645,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
               bad[b] |= 2u << (2 * t + 8 * h);
               pair[h][b] &= 0xffffu;
             }
-            pair[h][b] = half2_bits(__hmul2(bits_half2(pair[h][b]), sixteenth));
+            large |= (pair[h][b] & 0x7000u) == 0x7000u ? 0x10000u << (2 * t + 8 * h) : 0u;
+            large |= (pair[h][b] & 0x70000000u) == 0x70000000u ? 0x20000u << (2 * t + 8 * h) : 0u;
           }
+        }
+        large = __reduce_or_sync(0xffffffffu, large);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const __half2 key_by = __float2half2_rn((large >> (g + 8 * h)) & 1u ? 0.0625f : 1.0f);
+          const uint32_t two = large >> (16 + 2 * t + 8 * h);
+          const __half2 value_by = __floats2half2_rn(two & 1u ? 0.0625f : 1.0f, two & 2u ? 0.0625f : 1.0f);
+#pragma unroll
+          for (int b = 0; b < NB / 2; ++b)
+            now.key_scale[h][b] = half2_bits(__hmul2(bits_half2(now.key_scale[h][b]), key_by));
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            pair[h][b] = half2_bits(__hmul2(bits_half2(pair[h][b]), value_by));
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -648,7 +669,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           if (lane == 0)
             poison[(slot * kTileGroups + w) * NB + b] = static_cast<uint16_t>(bad[b]);
         }
-        flag |= any_bad ? 14u : 6u;
+        if (lane == 0)
+          held[slot * kTileGroups + w] = large;
+        flag |= (large & 0xffffu ? 2u : 0u) | (large >> 16 ? 4u : 0u) | (any_bad ? 8u : 0u);
       }
       if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
         return false;
