@@ -135,20 +135,6 @@ struct RawGroup {
   bool there;
 };
 
-template <int N>
-__device__ __forceinline__ void load_global(uint32_t (&w)[N], const uint8_t *p) {
-  if constexpr (N == 1)
-    w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-  else if constexpr (N == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    static_assert(N == 4, "words to a load");
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  }
-}
-
 template <int NB>
 __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
   using L = PrefillLayout<NB>;
@@ -569,16 +555,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const auto fetch = [&](RawGroup<NB> &raw) {
       raw.there = page >= 0 && static_cast<size_t>(page) < c.cache.pages;
       if (raw.there) {
+        // (ordinary loads: the read-only path is for memory that nobody writes while the kernel lives, and its life may begin
+        // while the call before it still fills the cache)
         const uint8_t *from = c.cache.data + static_cast<size_t>(page) * c.cache.page_stride +
                               (static_cast<size_t>(head) * per_page + place) * (18 * kDim);
-        load_global<NB>(raw.key[0], from + lane * NB * 4);
-        load_global<NB>(raw.key[1], from + 128 * NB + lane * NB * 4);
-        load_global<NB>(raw.value[0], from + 256 * NB + lane * NB * 4);
-        load_global<NB>(raw.value[1], from + 384 * NB + lane * NB * 4);
-        load_global<NB / 2>(raw.key_scale[0], from + 512 * NB + g * NB * 2);
-        load_global<NB / 2>(raw.key_scale[1], from + 512 * NB + (g + 8) * NB * 2);
-        load_global<NB>(raw.value_scale[0], from + 544 * NB + 2 * t * NB * 2);
-        load_global<NB>(raw.value_scale[1], from + 544 * NB + (2 * t + 8) * NB * 2);
+        load_words<NB>(raw.key[0], from + lane * NB * 4);
+        load_words<NB>(raw.key[1], from + 128 * NB + lane * NB * 4);
+        load_words<NB>(raw.value[0], from + 256 * NB + lane * NB * 4);
+        load_words<NB>(raw.value[1], from + 384 * NB + lane * NB * 4);
+        load_words<NB / 2>(raw.key_scale[0], from + 512 * NB + g * NB * 2);
+        load_words<NB / 2>(raw.key_scale[1], from + 512 * NB + (g + 8) * NB * 2);
+        load_words<NB>(raw.value_scale[0], from + 544 * NB + 2 * t * NB * 2);
+        load_words<NB>(raw.value_scale[1], from + 544 * NB + (2 * t + 8) * NB * 2);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
