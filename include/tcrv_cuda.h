@@ -405,7 +405,7 @@ int tcrv_cuda_gemm_q4_0_q8_0_static_scratch(size_t n, float *s, const uint8_t *v
  * given that with respect to y.  `positions` is int32, or int64 with TCRV_CUDA_ROPE_POSITIONS_I64.
  * Up to 4 tensors (queries and keys) share one launch and each token's angles; strides count
  * elements, the elements of a head are adjacent; y == x with equal strides works in place, any other
- * overlap does not. */
+ * overlap of an output is refused (with unequal strides all between a tensor's first and last byte counts). */
 #define TCRV_CUDA_ROPE_HALVES 1u
 #define TCRV_CUDA_ROPE_INVERSE 2u
 #define TCRV_CUDA_ROPE_POSITIONS_I64 4u

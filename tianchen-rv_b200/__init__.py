@@ -584,7 +584,7 @@ def rope(x, positions, freqs, halves: bool = False, magnitude: float = 1.0, inve
     """Rotates the first 2 * len(freqs) elements of every head of `x`, (tokens, heads, dim) float32,
     float16 or bfloat16, by positions[token] * freqs[pair]; pairs are neighbours, or with `halves` the
     same place of the two halves.  positions: int32 or int64.  `magnitude` multiplies the result.
-    `inverse` turns back: the gradient of x, given that of the result.  out=x works in place."""
+    `inverse` turns back: the gradient of x, given that of the result.  out=x works in place; other overlaps are refused."""
     return _native.rope(x, None, positions, freqs, halves, magnitude, inverse, out, None)
 
 

@@ -644,6 +644,58 @@ int check_kv_cache(const tcrv_cuda_kv_cache &c) {
   return TCRV_CUDA_OK;
 }
 
+// The rows of a (tokens, heads, dim) tensor; strides and sizes in bytes.
+struct HeadRows {
+  uintptr_t p;
+  int64_t tokens, heads, token, head, row;
+  uintptr_t end() const { return p + static_cast<uintptr_t>((tokens - 1) * token + (heads - 1) * head + row); }
+};
+
+// Whether two such tensors share memory.  Exact for equal strides (what lies in one buffer side by side, queries and keys of a
+// projection, has them); with others, all between the first and the last byte counts.  The stride of an axis of one does not matter.
+bool rows_overlap(HeadRows a, HeadRows b) {
+  if (a.p >= b.end() || b.p >= a.end())
+    return false;
+  a.head = a.heads == 1 ? b.head : a.head;
+  b.head = b.heads == 1 ? a.head : b.head;
+  if (a.tokens == 1)
+    a.token = b.token = 0;
+  if (a.token != b.token || a.head != b.head)
+    return true;
+  const int64_t distance = static_cast<int64_t>(b.p - a.p);
+  for (int64_t h = 1 - a.heads; h < b.heads; ++h) {
+    const int64_t at = distance + h * a.head;  // of b's row behind a's, the same token's; the nearest other token's:
+    int64_t t = a.token == 0 ? 0 : -at / a.token;
+    for (int64_t n = t - 1; n <= t + 1; ++n) {
+      const int64_t d = at + (n < 1 - a.tokens ? 1 - a.tokens : n > a.tokens - 1 ? a.tokens - 1 : n) * a.token;
+      if (d < a.row && -d < a.row)
+        return true;
+    }
+  }
+  return false;
+}
+
+// An output may be its own input, and nothing else that the call touches.
+bool rope_overlaps(int type, size_t tokens, size_t dim, const tcrv_cuda_rope_tensor *tensors, size_t count) {
+  const int64_t size = type == TCRV_CUDA_TYPE_F32 ? 4 : 2, n = static_cast<int64_t>(tokens), row = static_cast<int64_t>(dim) * size;
+  const auto input = [&](const tcrv_cuda_rope_tensor &t) {
+    return HeadRows{reinterpret_cast<uintptr_t>(t.x), n, static_cast<int64_t>(t.heads), static_cast<int64_t>(t.x_token_stride) * size, static_cast<int64_t>(t.x_head_stride) * size, row};
+  };
+  const auto output = [&](const tcrv_cuda_rope_tensor &t) {
+    return HeadRows{reinterpret_cast<uintptr_t>(t.y), n, static_cast<int64_t>(t.heads), static_cast<int64_t>(t.y_token_stride) * size, static_cast<int64_t>(t.y_head_stride) * size, row};
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const tcrv_cuda_rope_tensor &t = tensors[i];
+    if (t.heads == 0)
+      continue;
+    const bool in_place = t.x == t.y && (tokens == 1 || t.x_token_stride == t.y_token_stride) && (t.heads == 1 || t.x_head_stride == t.y_head_stride);
+    for (size_t j = 0; j < count; ++j)
+      if (tensors[j].heads != 0 && ((!(i == j && in_place) && rows_overlap(input(tensors[j]), output(t))) || (j < i && rows_overlap(output(tensors[j]), output(t)))))
+        return true;
+  }
+  return false;
+}
+
 int check_attention(const tcrv_cuda_attention_call &c) {
   const int st = check_kv_cache(c.cache);
   if (st != TCRV_CUDA_OK)
@@ -686,7 +738,7 @@ int tcrv_cuda_rope_rows(int type, size_t tokens, size_t dim, size_t n_rot, const
     return TCRV_CUDA_OK;
   if (heads * dim > (1u << 28))  // (a CTA counts the accesses of four tokens in 32 bits)
     return TCRV_CUDA_ERR_UNSUPPORTED;
-  if (!positions || (n_rot != 0 && !freqs))
+  if (!positions || (n_rot != 0 && !freqs) || rope_overlaps(type, tokens, dim, tensors, count))
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
   return launch_rope_rows(type, tokens, dim, n_rot, tensors, count, positions, freqs, magnitude, flags, as_stream(stream));
 }
