@@ -580,18 +580,54 @@ def rope_frequencies(n_rot: int, theta_base: float = 10000.0, scaling: str = "no
     return freqs
 
 
+_rope_function = None
+
+
+def _rope_recorded(*args):
+    """The rotation of tensors that require a gradient, as a node of torch's graph: backward is the rotation by the negative angle."""
+    global _rope_function
+    if _rope_function is None:
+        import torch
+
+        class Rope(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, q, k, positions, freqs, halves, magnitude, inverse):
+                ctx.set_materialize_grads(False)
+                ctx.save_for_backward(positions, freqs)
+                ctx.how = halves, magnitude, not inverse
+                return _native.rope(q, k, positions, freqs, halves, magnitude, inverse, None, None)
+
+            @staticmethod
+            def backward(ctx, *grads):
+                # (a broadcast gradient has no adjacent elements)
+                g = [x if need and x is not None else None for x, need in zip(grads, ctx.needs_input_grad)]
+                g = [x.contiguous() if x is not None and x.stride(-1) != 1 else x for x in g] + [None]
+                if g[0] is not None and g[1] is not None:
+                    g = rope_qk(g[0], g[1], *ctx.saved_tensors, *ctx.how)
+                else:
+                    g = [x if x is None else rope(x, *ctx.saved_tensors, *ctx.how) for x in g]
+                return g[0], g[1], None, None, None, None, None
+
+        _rope_function = Rope
+    return _rope_function.apply(*args)
+
+
 def rope(x, positions, freqs, halves: bool = False, magnitude: float = 1.0, inverse: bool = False, out=None):
     """Rotates the first 2 * len(freqs) elements of every head of `x`, (tokens, heads, dim) float32,
     float16 or bfloat16, by positions[token] * freqs[pair]; pairs are neighbours, or with `halves` the
     same place of the two halves.  positions: int32 or int64.  `magnitude` multiplies the result.
-    `inverse` turns back: the gradient of x, given that of the result.  out=x works in place; other overlaps are refused."""
-    return _native.rope(x, None, positions, freqs, halves, magnitude, inverse, out, None)
+    `inverse` turns back: the gradient of x, given that of the result, which torch's graph records by
+    itself where x requires one.  out=x works in place; other overlaps are refused, and any `out` where a
+    gradient would have to be recorded."""
+    y = _native.rope(x, None, positions, freqs, halves, magnitude, inverse, out, None)
+    return y if y is not None else _rope_recorded(x, None, positions, freqs, halves, magnitude, inverse)
 
 
 def rope_qk(q, k, positions, freqs, halves: bool = False, magnitude: float = 1.0, inverse: bool = False, out=None):
     """`rope` of queries and keys of the same tokens in one launch; `out` is a pair."""
     oq, ok = out if out is not None else (None, None)
-    return _native.rope(q, k, positions, freqs, halves, magnitude, inverse, oq, ok)
+    y = _native.rope(q, k, positions, freqs, halves, magnitude, inverse, oq, ok)
+    return y if y is not None else _rope_recorded(q, k, positions, freqs, halves, magnitude, inverse)
 
 
 class KvPlan(tuple):

@@ -8,6 +8,7 @@
 // them; a non-zero status goes to the package's `_check`, which raises TcrvCudaError.
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -582,12 +583,21 @@ PyObject *pair_of(at::Tensor a, at::Tensor b) {
   return r;
 }
 
-// rope(q, k or None, positions, freqs, halves, magnitude, inverse, out_q, out_k)
+// rope(q, k or None, positions, freqs, halves, magnitude, inverse, out_q, out_k); None where a gradient has to be recorded, which
+// the wrapper does
 TCRV_CALL(rope, 9) {
   const char *text = "x must be (tokens, heads, dim) with adjacent elements of a head";
   const at::Tensor &q = head_rows(a[0], text);
   const bool two = a[1] != Py_None;
   const at::Tensor &k = two ? head_rows(a[1], text) : q;
+  if (at::GradMode::is_enabled()) {
+    const auto recorded = [](PyObject *o) { return o != Py_None && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad(); };
+    const bool inputs = q.requires_grad() || k.requires_grad();
+    if ((inputs && (a[7] != Py_None || a[8] != Py_None)) || recorded(a[7]) || recorded(a[8]))
+      fail(PyExc_ValueError, "out= records no gradient: leave it out, or call under torch.no_grad()");
+    if (inputs)
+      Py_RETURN_NONE;
+  }
   const int type = activation_type(q);
   if (k.scalar_type() != q.scalar_type())
     fail(PyExc_TypeError, "queries and keys differ in type");
