@@ -496,7 +496,9 @@ int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream strea
  * A row that sees nothing gets zeros and lse = -inf; rows outside every request are left as they were.
  * Tokens behind `width` pages and tokens in pages outside the cache count as unseen.  `lse` (may be
  * null) gets the natural logarithm of each row's soft-max sum, [row][head].  Strides count elements,
- * the elements of a head are adjacent.  dim: 64, 96, 128, 192 or 256.
+ * the elements of a head are adjacent; out == q with equal strides works in place, any other overlap of
+ * the two is refused (with unequal strides all between first and last byte counts).  dim: 64, 96, 128,
+ * 192 or 256.
  * `workspace` holds the partial results of contexts that are split: 256-byte aligned,
  * tcrv_cuda_attention_q4_0_workspace_bytes(call) bytes (which ignores the call's pointers); nothing in
  * it outlives the call, and calls that may run at the same time need one each. */

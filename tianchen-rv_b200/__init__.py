@@ -695,8 +695,9 @@ def attention_q4_0(q, cache, block_table, kv_lens, first_rows=None, max_new: int
     first_rows), the last tokens of the kv_lens[r] that block_table[r] holds; a row sees the tokens up to
     its own, with `window` only the last `window` of them.  Rows from max_new on are left out, the others
     keep their positions.  scale: 1 / sqrt(dim).
-    A row that sees nothing gives zeros (lse -inf); rows outside every request are left as they were.
-    Returns out, or (out, lse) with lse (rows, heads) float32, the natural logarithm of the row's
+    A row that sees nothing gives zeros (lse -inf); rows outside every request are left as they were
+    (without `out`, unset).  out=q works in place; other overlaps of the two are refused.  No gradient is
+    recorded.  Returns out, or (out, lse) with lse (rows, heads) float32, the natural logarithm of the row's
     soft-max sum.  `workspace`: a uint8 tensor to use instead of a new one; calls that may overlap on the
     GPU need one each."""
     return _native.attention(q, cache, block_table, kv_lens, first_rows, max_new, scale, window, out, with_lse, workspace)

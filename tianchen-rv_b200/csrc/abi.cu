@@ -675,24 +675,32 @@ bool rows_overlap(HeadRows a, HeadRows b) {
   return false;
 }
 
+HeadRows head_rows(int type, const void *p, size_t tokens, size_t heads, size_t dim, size_t token_stride, size_t head_stride) {
+  const int64_t size = type == TCRV_CUDA_TYPE_F32 ? 4 : 2;
+  return {reinterpret_cast<uintptr_t>(p), static_cast<int64_t>(tokens), static_cast<int64_t>(heads), static_cast<int64_t>(token_stride) * size,
+          static_cast<int64_t>(head_stride) * size, static_cast<int64_t>(dim) * size};
+}
+
+// The same memory in the same order: an operation that reads a row before it writes it may work in place.
+bool same_rows(const HeadRows &a, const HeadRows &b) {
+  return a.p == b.p && (a.tokens == 1 || a.token == b.token) && (a.heads == 1 || a.head == b.head);
+}
+
 // An output may be its own input, and nothing else that the call touches.
 bool rope_overlaps(int type, size_t tokens, size_t dim, const tcrv_cuda_rope_tensor *tensors, size_t count) {
-  const int64_t size = type == TCRV_CUDA_TYPE_F32 ? 4 : 2, n = static_cast<int64_t>(tokens), row = static_cast<int64_t>(dim) * size;
-  const auto input = [&](const tcrv_cuda_rope_tensor &t) {
-    return HeadRows{reinterpret_cast<uintptr_t>(t.x), n, static_cast<int64_t>(t.heads), static_cast<int64_t>(t.x_token_stride) * size, static_cast<int64_t>(t.x_head_stride) * size, row};
-  };
-  const auto output = [&](const tcrv_cuda_rope_tensor &t) {
-    return HeadRows{reinterpret_cast<uintptr_t>(t.y), n, static_cast<int64_t>(t.heads), static_cast<int64_t>(t.y_token_stride) * size, static_cast<int64_t>(t.y_head_stride) * size, row};
-  };
+  HeadRows x[4], y[4];
+  size_t n = 0;
   for (size_t i = 0; i < count; ++i) {
     const tcrv_cuda_rope_tensor &t = tensors[i];
     if (t.heads == 0)
       continue;
-    const bool in_place = t.x == t.y && (tokens == 1 || t.x_token_stride == t.y_token_stride) && (t.heads == 1 || t.x_head_stride == t.y_head_stride);
-    for (size_t j = 0; j < count; ++j)
-      if (tensors[j].heads != 0 && ((!(i == j && in_place) && rows_overlap(input(tensors[j]), output(t))) || (j < i && rows_overlap(output(tensors[j]), output(t)))))
-        return true;
+    x[n] = head_rows(type, t.x, tokens, t.heads, dim, t.x_token_stride, t.x_head_stride);
+    y[n++] = head_rows(type, t.y, tokens, t.heads, dim, t.y_token_stride, t.y_head_stride);
   }
+  for (size_t i = 0; i < n; ++i)
+    for (size_t j = 0; j < n; ++j)
+      if ((!(i == j && same_rows(x[j], y[i])) && rows_overlap(x[j], y[i])) || (j < i && rows_overlap(y[j], y[i])))
+        return true;
   return false;
 }
 
@@ -824,6 +832,10 @@ int tcrv_cuda_attention_q4_0(const tcrv_cuda_attention_call *call, tcrv_cuda_str
   if (c.requests == 0 || c.rows == 0)
     return TCRV_CUDA_OK;
   if (!c.q || !c.out || !c.kv_lens || (c.width != 0 && !c.block_table) || (c.requests > 1 && c.table_stride < c.width))
+    return TCRV_CUDA_ERR_INVALID_ARGUMENT;
+  const HeadRows q = head_rows(c.type, c.q, c.rows, c.heads, c.cache.dim, c.q_row_stride, c.q_head_stride),
+                 out = head_rows(c.type, c.out, c.rows, c.heads, c.cache.dim, c.out_row_stride, c.out_head_stride);
+  if (!same_rows(q, out) && rows_overlap(q, out))
     return TCRV_CUDA_ERR_INVALID_ARGUMENT;
   if (!c.workspace || reinterpret_cast<uintptr_t>(c.workspace) % 256 != 0 || c.workspace_bytes < attention_workspace_bytes(c))
     return TCRV_CUDA_ERR_WORKSPACE;
