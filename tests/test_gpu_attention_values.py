@@ -131,6 +131,32 @@ def test_prompts_on_average(cuda, pkg, kind, n, new, dim):
     rms.check(got, lse, d, kind, True)
 
 
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("n,new,dim,window", [(60, 60, 128, 0), (400, 300, 128, 6), (17, 17, 64, 0), (3000, 40, 64, 3), (700, 128, 128, 0)])
+def test_the_soft_max_sum_of_prompts_is_f32(cuda, pkg, kind, n, new, dim, window):
+    """The result is 16 bits wide, its logarithm of the sum is not: keys count with all the bits of scale times quant.
+    A score is a sum of up to 2 * 8 steps of 16 products and the sum so far, each aligned and cut at 2^-24 of the largest: 272 cuts,
+    of terms and partial sums the size of the root of the terms' squares.  2^-18 allows for 2^x, the sum's additions and the logarithm."""
+    d, got, lse = prompt_case(cuda, pkg, kind, n, new, 8, 2, dim, ordinary, ordinary, seed=n, window=window)
+    rms.check(got, lse, d, kind, True)
+    off = lse.double().cpu().numpy() - d["lse"]
+    allowed = 272 * 2.0 ** -24 * d["spread"] + 2.0 ** -18 + np.abs(d["lse"]) * 2.0 ** -22
+    ratio = ((off / allowed) ** 2).mean()
+    assert ratio <= 1, f"mean square error of lse {ratio:.3g} of the allowed"
+
+
+@pytest.mark.parametrize("kind", HALF)
+@pytest.mark.parametrize("n,new,dim", [(700, 400, 128), (1500, 33, 128), (300, 300, 64)])
+def test_prompts_without_the_sum(cuda, pkg, kind, n, new, dim):
+    rng = np.random.default_rng(n)
+    cache, table = build(rng, [n], 2, 32, dim, ordinary(rng), ordinary(rng))
+    q, q64 = tensor(cuda, rng.standard_normal((new, 4, dim)), kind)
+    got = pkg.attention_q4_0(q, cuda.from_numpy(cache).cuda(), cuda.from_numpy(table.astype(np.int32)).cuda(), ints(cuda, [n]),
+                             first_rows=ints(cuda, [0, new]), max_new=new)
+    pkg.check_device_errors()
+    rms.check(got, None, rms.definition(q64, cache, table, [n], [0, new], dim ** -0.5), kind, True)
+
+
 SMALL = {"float16": (6.2e-5, 1e-4), "bfloat16": (1e-5, 2e-5)}  # (a scale below 2^-14 times a quant is a whole number of fp16's steps)
 
 

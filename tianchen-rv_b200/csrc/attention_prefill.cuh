@@ -13,8 +13,12 @@
 // of eight 818 us; a thread to a row, one warpgroup to a tile, 459 (with the tiles' passes taking turns 510); half of the
 // exponentials by a polynomial 517, for the schedulers have no cycles to spare for it.
 //
-// Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (2^-12 relative): their f32 sums could not be
-// scaled block by block without reading S and O once for every block of 32.  Query rows are fp16 after a power of two
+// Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (half a step of 2^-11): their f32 sums could not be
+// scaled block by block without reading S and O once for every block of 32.  What the keys' rounding leaves out is a multiple of
+// the scale's last place, hence an fp16 number itself: calls with an f32 output (lse) or fp16 ones add its product to S, which then
+// has all the bits of the keys (kExact; without it lse was off by 1e-4 over the root of the tokens seen, and fp16 results by 1.7
+// times their own rounding; 4 prompts of up to 2048 tokens behind 2048, bf16: 517 us with it, 451 without).  A bf16 result's own
+// rounding is 8 times the keys'.  Query rows are fp16 after a power of two
 // (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A token with a scale so large that
 // its values leave fp16 is held at 1/16 and made good in S or in P.  The running maximum that P is relative to follows the
 // true one only when that has grown by more than 2^8: then O is rescaled, otherwise P just has values up to 2^8.
@@ -61,21 +65,24 @@ struct PrefillLayout {
   static constexpr int kValueBytes = kTileTokens / 64 * kDim * 128;  // D x 128 tokens, K-major
   static constexpr int kQuery = 0;
   static constexpr int kKey = kQuery + 2 * kKeyBytes;
-  static constexpr int kValue = kKey + 2 * kKeyBytes;
+  static constexpr int kKeyLow = kKey + 2 * kKeyBytes;           // what the fp16 keys leave out, one stage
+  static constexpr int kValue = kKeyLow + kKeyBytes;
   static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
   static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group][block]: tokens whose value scale is no number
   static constexpr int kHeld = kPoison + kSlots * kTileGroups * NB * 2;     // u32 [slot][group]: tokens held at 1/16, keys, values << 16
-  static constexpr int kBadRows = kHeld + kSlots * kTileGroups * 4;         // u8 [tile][half][row]: blocks of which it sees such a token
-  static constexpr int kBars = kBadRows + 2 * 2 * 128;
-  static constexpr int kBarCount = 20;
+  static constexpr int kBadRows = kHeld + kSlots * kTileGroups * 4;         // u8 [half][row]: blocks of which it sees such a token, tile 1's << 4
+  static constexpr int kBars = kBadRows + 2 * 128;
+  static constexpr int kBarCount = 22;
   static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
   static constexpr int kTmem = kTops + 2 * 2 * 128 * 4;
   static constexpr int kAbort = kTmem + 4;
-  static constexpr int kBytes = kAbort + 4 + 1024;  // (the base is rounded up to 1024)
+  static constexpr int kBytes = kAbort + 4;
+  static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
+  static_assert(NB <= 4 && kBars % 8 == 0, "blocks of a row in half a byte; barriers");
 };
 
 // barriers
-enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15, kBarDrain = 19 };
+enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15, kBarDrain = 19, kBarLowFull = 20, kBarLowFree = 21 };
 
 // kind::f16, fp16 A and B (both K-major), f32 D.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
@@ -135,12 +142,13 @@ struct RawGroup {
   bool there;
 };
 
-template <int NB>
+// kExact: scores of keys with all their bits (two products), see above.
+template <int NB, bool kExact>
 __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
   using L = PrefillLayout<NB>;
   constexpr int kDim = L::kDim;
-  extern __shared__ uint8_t prefill_smem[];
-  uint8_t *smem = prefill_smem + ((1024u - (smem_addr(prefill_smem) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t prefill_smem[];  // (the operands' swizzle goes by address bits; no room to round up)
+  uint8_t *smem = prefill_smem;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
   uint32_t *tmem_word = reinterpret_cast<uint32_t *>(smem + L::kTmem);
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + L::kAbort);
@@ -152,6 +160,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_enter();
+  if ((smem_addr(smem) & 1023u) != 0) {  // (never, as long as dynamic shared memory is given the alignment that it asks for)
+    if (threadIdx.x == 0)
+      raise_device_error(p.errors, kDevErrSharedAlignment);
+    return;
+  }
   // ---- what this CTA does: the longest row blocks come first
   const uint32_t kv_heads = static_cast<uint32_t>(c.cache.kv_heads);
   uint32_t id = blockIdx.x;
@@ -197,6 +210,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     for (int i = 0; i < 4; ++i)
       mbar_init(&bars[kBarPair + i], 2);
     mbar_init(&bars[kBarDrain], 1);
+    mbar_init(&bars[kBarLowFull], kQuantWarps);
+    mbar_init(&bars[kBarLowFree], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -230,7 +245,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const int32_t group = static_cast<int32_t>(p.group);
     float *tops = reinterpret_cast<float *>(smem + L::kTops);
     int lifts = 0;  // powers of the queries of this thread's row in the two tiles, a byte each
-    bad_rows[half * 128 + row] = bad_rows[(2 + half) * 128 + row] = 0;
+    bad_rows[half * 128 + row] = 0;
     {
       // ---- the query operand, tile `half`: 32 rows of it, in the key operand's order of elements, times a power of two that
       // lifts the largest element into [2^14, 2^15).  kDim / 8 lanes to a row, eight elements to a lane.
@@ -441,7 +456,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
             for (int b = 0; b < NB; ++b)
               blocks |= (poison[(slot * kTileGroups + 4 * half + h) * NB + b] & seen) ? 1u << b : 0u;
             if (blocks)
-              bad_rows[(tile * 2 + half) * 128 + row] |= static_cast<uint8_t>(blocks);
+              bad_rows[half * 128 + row] |= static_cast<uint8_t>(blocks << (4 * tile));
           }
         }
       }
@@ -478,7 +493,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       float l = st.l;
       if (wait(kBarPair + (warp & 3), steps + 1 + tile))
         l = half == 0 ? l + exchange[128 + row] : exchange[row] + l;
-      const uint32_t bad = bad_rows[tile * 2 * 128 + row] | bad_rows[(tile * 2 + 1) * 128 + row];
+      const uint32_t bad = static_cast<uint32_t>(bad_rows[row] | bad_rows[128 + row]) >> (4 * tile);
       const int32_t pair = pair0 + tile * kTileRows + row, token = pair / group;
       const size_t q_head = static_cast<size_t>(head) * group + (pair - token * group);
       const size_t at = static_cast<size_t>(q.first_row + token) * c.out_row_stride + q_head * c.out_head_stride;
@@ -683,6 +698,30 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&bars[kBarKeyFull + stage]);
+      // ---- what the fp16 keys leave out, scale * quant less its rounding: exact, for it is a multiple of the scale's last place
+      if constexpr (kExact) {
+        if (j >= 1 && !wait(kBarLowFree, j - 1))
+          return false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint32_t word = now.key[h][b];
+            asm volatile("" : "+r"(word));  // (unpacked again: kept from above, it would take 32 registers)
+            const __half2 scale = bits_half2(__byte_perm(now.key_scale[h][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
+            const auto rest = [&](uint32_t n) {
+              const __half2 q = bits_half2(n);
+              return half2_bits(__hfma2(q, scale, __hneg2(__hmul2(q, scale))));
+            };
+            const uint4 v = make_uint4(rest(low_nibbles(word)), rest(low_nibbles(word >> 8)), rest(high_nibbles(word)), rest(high_nibbles(word >> 8)));
+            *reinterpret_cast<uint4 *>(((b & 1) ? key_odd : key_even) + (L::kKeyLow - L::kKey) + (b >> 1) * L::kPanel + h * 1024) = v;
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars[kBarLowFull]);
+      }
       // ---- values, transposed: row n of the operand is an element, its columns the tokens
       if (j >= 2 && !wait(kBarValueFree + stage, (j >> 1) - 1))
         return false;
@@ -733,15 +772,27 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0), columns = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint32_t kScoreDesc = umma_idesc_f16(kTileRows, kTileTokens), kSumDesc = umma_idesc_f16(kTileRows, kDim);
     const bool leader = elect_one();
-    const auto score = [&](int tile, int stage) {
-      const uint32_t a = desc_low(base + L::kQuery + tile * L::kKeyBytes), b = desc_low(base + L::kKey + stage * L::kKeyBytes);
-      umma_f16_ss<false>(columns + tile * 128, a, b, kScoreDesc);
+    const auto score = [&](int tile, int stage, bool last) {  // the small parts first: their place is free soonest
+      const uint32_t a = desc_low(base + L::kQuery + tile * L::kKeyBytes), low = desc_low(base + L::kKeyLow), b = desc_low(base + L::kKey + stage * L::kKeyBytes);
+      if constexpr (kExact) {
+        umma_f16_ss<false>(columns + tile * 128, a, low, kScoreDesc);
+#pragma unroll
+        for (int k = 1; k < kDim / 16; ++k) {
+          const uint32_t at = (k / 4) * (L::kPanel >> 4) + (k % 4) * 2;
+          umma_f16_ss<true>(columns + tile * 128, a + at, low + at, kScoreDesc);
+        }
+        if (last)
+          umma_commit(&bars[kBarLowFree]);
+      }
+      umma_f16_ss<kExact>(columns + tile * 128, a, b, kScoreDesc);
 #pragma unroll
       for (int k = 1; k < kDim / 16; ++k) {
         const uint32_t at = (k / 4) * (L::kPanel >> 4) + (k % 4) * 2;
         umma_f16_ss<true>(columns + tile * 128, a + at, b + at, kScoreDesc);
       }
       umma_commit(&bars[kBarScores + tile]);
+      if (last)
+        umma_commit(&bars[kBarKeyFree + stage]);
     };
     const auto sum = [&](int tile, int stage, bool add) {
       const uint32_t b = desc_low(base + L::kValue + stage * L::kValueBytes);
@@ -752,12 +803,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       }
       umma_commit(&bars[kBarSums + tile]);
     };
-    bool good = wait(kBarQuery, 0) && wait(kBarKeyFull, 0);
+    bool good = wait(kBarQuery, 0) && wait(kBarKeyFull, 0) && (!kExact || wait(kBarLowFull, 0));
     tcgen05_fence_after_thread_sync();
     if (good && leader) {
       for (int i = 0; i < tiles_q; ++i)
-        score(i, 0);
-      umma_commit(&bars[kBarKeyFree]);
+        score(i, 0, i == tiles_q - 1);
     }
 #pragma unroll 1
     for (int j = 0; j < tiles && good; ++j) {
@@ -765,20 +815,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       good = wait(kBarValueFull + stage, j >> 1);
       for (int i = 0; i < tiles_q && good; ++i) {
         good = wait(kBarWeights + i, j);
-        if (i == 0 && good && j + 1 < tiles)
-          good = wait(kBarKeyFull + next, (j + 1) >> 1);
         tcgen05_fence_after_thread_sync();
         if (good && leader) {
           sum(i, stage, j > 0);
           if (i == tiles_q - 1)
             umma_commit(&bars[kBarValueFree + stage]);
-          if (j + 1 < tiles) {
-            score(i, next);
-            if (i == tiles_q - 1)
-              umma_commit(&bars[kBarKeyFree + next]);
-          }
         }
         __syncwarp();
+        if (j + 1 < tiles) {
+          if (i == 0 && good)
+            good = wait(kBarKeyFull + next, (j + 1) >> 1) && (!kExact || wait(kBarLowFull, j + 1));
+          tcgen05_fence_after_thread_sync();
+          if (good && leader)
+            score(i, next, i == tiles_q - 1);
+          __syncwarp();
+        }
       }
     }
     if (!good) {  // products on their way end before their memory goes back

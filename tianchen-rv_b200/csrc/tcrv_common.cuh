@@ -25,6 +25,7 @@ struct DeviceErrorWords {
   int **mirror;
 };
 constexpr int kDevErrBarrierTimeout = 1;
+constexpr int kDevErrSharedAlignment = 2;  // dynamic shared memory off the boundary that a kernel asked for
 
 // What a kernel calls when one of its bounded waits expires.
 __device__ __forceinline__ void raise_device_error(const DeviceErrorWords &w, int code) {
