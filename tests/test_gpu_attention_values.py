@@ -157,6 +157,17 @@ def test_prompts_without_the_sum(cuda, pkg, kind, n, new, dim):
     rms.check(got, None, rms.definition(q64, cache, table, [n], [0, new], dim ** -0.5), kind, True)
 
 
+@pytest.mark.parametrize("n,new,dim", [(200, 150, 128), (90, 90, 64), (2000, 34, 128)])
+def test_values_of_fp16_prompts_are_whole(cuda, pkg, n, new, dim):
+    """Keys of zero and a window of 16: weights of 1, sums and a sixteenth of them without rounding, so that a result is the mean of 16
+    values rounded once."""
+    none = lambda rng: lambda r, shape: np.zeros(shape)  # noqa: E731
+    d, got, lse = prompt_case(cuda, pkg, "float16", n, new, 4, 2, dim, none, ordinary, seed=n, window=16)
+    full = max(0, 15 - (n - new))  # rows from here on see 16 tokens
+    assert np.array_equal(got[full:].cpu().numpy(), d["out"][full:].astype(np.float32).astype(np.float16))
+    assert (np.abs(lse[full:].cpu().numpy() - np.log(16)) <= 2.0 ** -21).all()
+
+
 SMALL = {"float16": (6.2e-5, 1e-4), "bfloat16": (1e-5, 2e-5)}  # (a scale below 2^-14 times a quant is a whole number of fp16's steps)
 
 

@@ -124,7 +124,7 @@ int launch_dim(const ColumnParams &p, const Shape &s, cudaStream_t stream) {
                             : launch_tiles<NB, kTwoTerms>(p, s, stream);
 }
 
-template <int NB, bool kExact>
+template <int NB, int MODE>
 int launch_prefill(const tcrv_cuda_attention_call &c, const Shape &s, const DeviceErrorWords &errors, cudaStream_t stream) {
   if (s.parts > 0x7fffffff)
     return TCRV_CUDA_ERR_UNSUPPORTED;
@@ -135,13 +135,13 @@ int launch_prefill(const tcrv_cuda_attention_call &c, const Shape &s, const Devi
   p.min_rows = static_cast<int32_t>(kPrefillRows);
   p.splits = s.splits;
   p.errors = errors;
-  constexpr size_t smem = PrefillLayout<NB>::kBytes;
+  constexpr size_t smem = PrefillLayout<NB, MODE>::kBytes;
   static Configured state;
-  const int st = configure(state, reinterpret_cast<const void *>(prefill_kernel<NB, kExact>), smem, kPrefillThreads,
+  const int st = configure(state, reinterpret_cast<const void *>(prefill_kernel<NB, MODE>), smem, kPrefillThreads,
                            128 * (2 * kSoftmaxRegs + 2 * kQuantRegs + kProductRegs));
   if (st != TCRV_CUDA_OK)
     return st;
-  TCRV_CUDA_TRY(launch_pdl(prefill_kernel<NB, kExact>, dim3(static_cast<unsigned>(s.parts)), kPrefillThreads, smem, stream, p));
+  TCRV_CUDA_TRY(launch_pdl(prefill_kernel<NB, MODE>, dim3(static_cast<unsigned>(s.parts)), kPrefillThreads, smem, stream, p));
   if (s.splits > 1) {
     const dim3 grid(2 * kTileRows / 8, static_cast<unsigned>(s.parts / s.splits));
     TCRV_CUDA_TRY(launch_pdl(prefill_combine_kernel<NB>, grid, 256, 0, stream, p, static_cast<uint32_t>(s.parts)));
@@ -163,10 +163,14 @@ int launch_attention_q4_0(const tcrv_cuda_attention_call &c, cudaStream_t stream
   if (st != TCRV_CUDA_OK)
     return st;
   if (s.prefill) {
-    const bool exact = c.lse != nullptr || c.type == TCRV_CUDA_TYPE_F16;  // (bf16 results hide the keys' rounding)
-    const int rc = c.cache.dim == 64 ? exact ? launch_prefill<2, true>(c, s, p.errors, stream) : launch_prefill<2, false>(c, s, p.errors, stream)
-                   : exact           ? launch_prefill<4, true>(c, s, p.errors, stream)
-                                     : launch_prefill<4, false>(c, s, p.errors, stream);
+    // as exact as the outputs show: fp16 results both roundings, an f32 lse that of the keys, bf16 results neither
+    const auto launch = [&](auto dim) {
+      constexpr int kBlocks = decltype(dim)::value;
+      return c.type == TCRV_CUDA_TYPE_F16 ? launch_prefill<kBlocks, kExactAll>(c, s, p.errors, stream)
+             : c.lse != nullptr           ? launch_prefill<kBlocks, kExactKeys>(c, s, p.errors, stream)
+                                          : launch_prefill<kBlocks, kRounded>(c, s, p.errors, stream);
+    };
+    const int rc = c.cache.dim == 64 ? launch(std::integral_constant<int, 2>()) : launch(std::integral_constant<int, 4>());
     if (rc != TCRV_CUDA_OK)
       return rc;
   }

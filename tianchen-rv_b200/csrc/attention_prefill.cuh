@@ -13,15 +13,16 @@
 // of eight 818 us; a thread to a row, one warpgroup to a tile, 459 (with the tiles' passes taking turns 510); half of the
 // exponentials by a polynomial 517, for the schedulers have no cycles to spare for it.
 //
-// Numbers.  Key and value operands are d * (n - 8) rounded to fp16 once (half a step of 2^-11): their f32 sums could not be
-// scaled block by block without reading S and O once for every block of 32.  What the keys' rounding leaves out is a multiple of
-// the scale's last place, hence an fp16 number itself: calls with an f32 output (lse) or fp16 ones add its product to S, which then
-// has all the bits of the keys (kExact; without it lse was off by 1e-4 over the root of the tokens seen, and fp16 results by 1.7
-// times their own rounding; 4 prompts of up to 2048 tokens behind 2048, bf16: 517 us with it, 451 without).  A bf16 result's own
-// rounding is 8 times the keys'.  Query rows are fp16 after a power of two
-// (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A token with a scale so large that
-// its values leave fp16 is held at 1/16 and made good in S or in P.  The running maximum that P is relative to follows the
-// true one only when that has grown by more than 2^8: then O is rescaled, otherwise P just has values up to 2^8.
+// Numbers.  Key and value operands are d * (n - 8) rounded to fp16 (half a step of 2^-11), for their f32 sums could not be scaled
+// block by block without reading S and O once for every block of 32.  What the rounding leaves out is a multiple of the scale's
+// last place, hence an fp16 number: where an output shows it, it is a second operand whose product goes into the same sums.  So
+//   fp16 results: keys and values whole (with both rounded, results were off by 1.7 times their own rounding);
+//   bf16 results with lse, which is f32: keys whole (rounded, lse was off by 1e-4 over the root of the tokens seen);
+//   bf16 results alone, whose own rounding is 8 times as large: both rounded.
+// Query rows are fp16 after a power of two (exact for both types), weights are rounded to fp16; S, O, maximum and sum are f32.  A
+// token with a scale so large that its values leave fp16 is held at 1/16 and made good in S or in P (its other blocks lose what lies
+// below 2^-20).  The running maximum that P is relative to follows the true one only when that has grown by more than 2^8: then O is
+// rescaled, otherwise P just has values up to 2^8.
 #pragma once
 
 #include <type_traits>
@@ -57,22 +58,29 @@ inline size_t prefill_workspace_bytes(size_t parts, size_t dim) {
   return prefill_sums_offset(parts) + parts * 2 * kTileRows * dim * sizeof(float);
 }
 
-template <int NB>
+// What the products see of keys and values.
+constexpr int kRounded = 0;    // both rounded to fp16
+constexpr int kExactKeys = 1;  // keys whole, as two terms with a product each
+constexpr int kExactAll = 2;   // values too
+
+template <int NB, int MODE>
 struct PrefillLayout {
   static constexpr int kDim = 32 * NB;
   static constexpr int kPanel = 128 * 128;                       // 128 rows of 128 bytes
   static constexpr int kKeyBytes = kDim / 64 * kPanel;           // 128 tokens x D, K-major
   static constexpr int kValueBytes = kTileTokens / 64 * kDim * 128;  // D x 128 tokens, K-major
   static constexpr int kQuery = 0;
+  static constexpr int kKeyStages = MODE == kExactAll ? 1 : 2;    // (what shared memory has room for)
   static constexpr int kKey = kQuery + 2 * kKeyBytes;
-  static constexpr int kKeyLow = kKey + 2 * kKeyBytes;           // what the fp16 keys leave out, one stage
-  static constexpr int kValue = kKeyLow + kKeyBytes;
-  static constexpr int kFlags = kValue + 2 * kValueBytes;        // u8 [slot][group]
+  static constexpr int kKeyLow = kKey + kKeyStages * kKeyBytes;   // second terms, one stage
+  static constexpr int kValue = kKeyLow + (MODE != kRounded ? kKeyBytes : 0);
+  static constexpr int kValueLow = kValue + 2 * kValueBytes;
+  static constexpr int kFlags = kValueLow + (MODE == kExactAll ? kValueBytes : 0);  // u8 [slot][group]
   static constexpr int kPoison = kFlags + kSlots * kTileGroups;  // u16 [slot][group][block]: tokens whose value scale is no number
   static constexpr int kHeld = kPoison + kSlots * kTileGroups * NB * 2;     // u32 [slot][group]: tokens held at 1/16, keys, values << 16
   static constexpr int kBadRows = kHeld + kSlots * kTileGroups * 4;         // u8 [half][row]: blocks of which it sees such a token, tile 1's << 4
   static constexpr int kBars = kBadRows + 2 * 128;
-  static constexpr int kBarCount = 22;
+  static constexpr int kBarCount = 24;
   static constexpr int kTops = kBars + kBarCount * 8;            // f32 [step parity][half][row]
   static constexpr int kTmem = kTops + 2 * 2 * 128 * 4;
   static constexpr int kAbort = kTmem + 4;
@@ -82,7 +90,7 @@ struct PrefillLayout {
 };
 
 // barriers
-enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15, kBarDrain = 19, kBarLowFull = 20, kBarLowFree = 21 };
+enum { kBarQuery = 0, kBarKeyFull = 1, kBarKeyFree = 3, kBarValueFull = 5, kBarValueFree = 7, kBarScores = 9, kBarWeights = 11, kBarSums = 13, kBarPair = 15, kBarDrain = 19, kBarKeyLowFull = 20, kBarKeyLowFree = 21, kBarValueLowFull = 22, kBarValueLowFree = 23 };
 
 // kind::f16, fp16 A and B (both K-major), f32 D.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
@@ -133,6 +141,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// What quant * scale loses when it is rounded to fp16: exact, for it is a multiple of the scale's last place.
+__device__ __forceinline__ uint32_t rounded_off(uint32_t quants, __half2 scale) {
+  const __half2 n = bits_half2(quants);
+  return half2_bits(__hfma2(n, scale, __hneg2(__hmul2(n, scale))));
+}
+
 // One lane's share of a group as it lies in the cache.
 template <int NB>
 struct RawGroup {
@@ -142,10 +156,9 @@ struct RawGroup {
   bool there;
 };
 
-// kExact: scores of keys with all their bits (two products), see above.
-template <int NB, bool kExact>
+template <int NB, int MODE>
 __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
-  using L = PrefillLayout<NB>;
+  using L = PrefillLayout<NB, MODE>;
   constexpr int kDim = L::kDim;
   extern __shared__ __align__(1024) uint8_t prefill_smem[];  // (the operands' swizzle goes by address bits; no room to round up)
   uint8_t *smem = prefill_smem;
@@ -210,8 +223,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     for (int i = 0; i < 4; ++i)
       mbar_init(&bars[kBarPair + i], 2);
     mbar_init(&bars[kBarDrain], 1);
-    mbar_init(&bars[kBarLowFull], kQuantWarps);
-    mbar_init(&bars[kBarLowFree], 1);
+    mbar_init(&bars[kBarKeyLowFull], kQuantWarps);
+    mbar_init(&bars[kBarKeyLowFree], 1);
+    mbar_init(&bars[kBarValueLowFull], kQuantWarps);
+    mbar_init(&bars[kBarValueLowFree], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -600,7 +615,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     uint8_t *const value_first = smem + L::kValue + (w >> 2) * (kDim * 128) + g * 128 + t * 4 + ((((w & 3) * 2) ^ g) << 4);
     uint8_t *const value_second = smem + L::kValue + (w >> 2) * (kDim * 128) + g * 128 + t * 4 + ((((w & 3) * 2 + 1) ^ g) << 4);
     const auto convert = [&](RawGroup<NB> &now, int j) -> bool {
-      const int stage = j & 1, slot = j % kSlots;
+      const int stage = j & 1, key_stage = j % L::kKeyStages, slot = j % kSlots;
       // ---- scales: of values, two tokens side by side; none for tokens behind the context; large ones are seen to
       uint32_t pair[2][NB];
       uint32_t some = 0;
@@ -676,7 +691,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           held[slot * kTileGroups + w] = large;
         flag |= (large & 0xffffu ? 2u : 0u) | (large >> 16 ? 4u : 0u) | (any_bad ? 8u : 0u);
       }
-      if (j >= 2 && !wait(kBarKeyFree + stage, (j >> 1) - 1))
+      if (j >= L::kKeyStages && !wait(kBarKeyFree + key_stage, j / L::kKeyStages - 1))
         return false;
       if (lane == 0)
         flags[slot * kTileGroups + w] = static_cast<uint8_t>(flag);
@@ -691,16 +706,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
                                      half2_bits(__hmul2(bits_half2(low_nibbles(word >> 8)), scale)),
                                      half2_bits(__hmul2(bits_half2(high_nibbles(word)), scale)),
                                      half2_bits(__hmul2(bits_half2(high_nibbles(word >> 8)), scale)));
-          *reinterpret_cast<uint4 *>(((b & 1) ? key_odd : key_even) + stage * L::kKeyBytes + (b >> 1) * L::kPanel + h * 1024) = v;
+          *reinterpret_cast<uint4 *>(((b & 1) ? key_odd : key_even) + key_stage * L::kKeyBytes + (b >> 1) * L::kPanel + h * 1024) = v;
         }
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0)
-        mbar_arrive(&bars[kBarKeyFull + stage]);
-      // ---- what the fp16 keys leave out, scale * quant less its rounding: exact, for it is a multiple of the scale's last place
-      if constexpr (kExact) {
-        if (j >= 1 && !wait(kBarLowFree, j - 1))
+        mbar_arrive(&bars[kBarKeyFull + key_stage]);
+      // ---- what the fp16 keys leave out
+      if constexpr (MODE != kRounded) {
+        if (j >= 1 && !wait(kBarKeyLowFree, j - 1))
           return false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -709,18 +724,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
             uint32_t word = now.key[h][b];
             asm volatile("" : "+r"(word));  // (unpacked again: kept from above, it would take 32 registers)
             const __half2 scale = bits_half2(__byte_perm(now.key_scale[h][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
-            const auto rest = [&](uint32_t n) {
-              const __half2 q = bits_half2(n);
-              return half2_bits(__hfma2(q, scale, __hneg2(__hmul2(q, scale))));
-            };
-            const uint4 v = make_uint4(rest(low_nibbles(word)), rest(low_nibbles(word >> 8)), rest(high_nibbles(word)), rest(high_nibbles(word >> 8)));
+            const uint4 v = make_uint4(rounded_off(low_nibbles(word), scale), rounded_off(low_nibbles(word >> 8), scale),
+                                       rounded_off(high_nibbles(word), scale), rounded_off(high_nibbles(word >> 8), scale));
             *reinterpret_cast<uint4 *>(((b & 1) ? key_odd : key_even) + (L::kKeyLow - L::kKey) + (b >> 1) * L::kPanel + h * 1024) = v;
           }
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0)
-          mbar_arrive(&bars[kBarLowFull]);
+          mbar_arrive(&bars[kBarKeyLowFull]);
       }
       // ---- values, transposed: row n of the operand is an element, its columns the tokens
       if (j >= 2 && !wait(kBarValueFree + stage, (j >> 1) - 1))
@@ -744,6 +756,29 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&bars[kBarValueFull + stage]);
+      // ---- what the fp16 values leave out
+      if constexpr (MODE == kExactAll) {
+        if (j >= 1 && !wait(kBarValueLowFree, j - 1))
+          return false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint32_t word = now.value[h][b];
+            asm volatile("" : "+r"(word));
+            const __half2 scale = bits_half2(pair[h][b]);
+            const uint32_t v[4] = {rounded_off(low_nibbles(word), scale), rounded_off(low_nibbles(word >> 8), scale),
+                                   rounded_off(high_nibbles(word), scale), rounded_off(high_nibbles(word >> 8), scale)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint32_t *>((h ? value_second : value_first) + (L::kValueLow - L::kValue) + (b * 4 + k) * 1024) = v[k];
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars[kBarValueLowFull]);
+      }
       return true;
     };
     // Two tiles' groups are on their way; each register set is filled again as soon as it has been used, without a copy.
@@ -772,9 +807,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0), columns = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint32_t kScoreDesc = umma_idesc_f16(kTileRows, kTileTokens), kSumDesc = umma_idesc_f16(kTileRows, kDim);
     const bool leader = elect_one();
-    const auto score = [&](int tile, int stage, bool last) {  // the small parts first: their place is free soonest
-      const uint32_t a = desc_low(base + L::kQuery + tile * L::kKeyBytes), low = desc_low(base + L::kKeyLow), b = desc_low(base + L::kKey + stage * L::kKeyBytes);
-      if constexpr (kExact) {
+    // (second terms first: their place is free soonest)
+    const auto score = [&](int tile, int stage, bool last) {
+      const uint32_t a = desc_low(base + L::kQuery + tile * L::kKeyBytes), b = desc_low(base + L::kKey + stage * L::kKeyBytes);
+      if constexpr (MODE != kRounded) {
+        const uint32_t low = desc_low(base + L::kKeyLow);
         umma_f16_ss<false>(columns + tile * 128, a, low, kScoreDesc);
 #pragma unroll
         for (int k = 1; k < kDim / 16; ++k) {
@@ -782,9 +819,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
           umma_f16_ss<true>(columns + tile * 128, a + at, low + at, kScoreDesc);
         }
         if (last)
-          umma_commit(&bars[kBarLowFree]);
+          umma_commit(&bars[kBarKeyLowFree]);
       }
-      umma_f16_ss<kExact>(columns + tile * 128, a, b, kScoreDesc);
+      umma_f16_ss<MODE != kRounded>(columns + tile * 128, a, b, kScoreDesc);
 #pragma unroll
       for (int k = 1; k < kDim / 16; ++k) {
         const uint32_t at = (k / 4) * (L::kPanel >> 4) + (k % 4) * 2;
@@ -794,16 +831,29 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
       if (last)
         umma_commit(&bars[kBarKeyFree + stage]);
     };
-    const auto sum = [&](int tile, int stage, bool add) {
+    const auto sum = [&](int tile, int stage, bool add, bool last) {
       const uint32_t b = desc_low(base + L::kValue + stage * L::kValueBytes);
+      if constexpr (MODE == kExactAll) {
+        const uint32_t low = desc_low(base + L::kValueLow);
+#pragma unroll
+        for (int k = 0; k < kTileTokens / 16; ++k) {
+          const uint32_t at = (k / 4) * ((kDim * 128) >> 4) + (k % 4) * 2;
+          umma_f16_ts(columns + 256 + tile * kDim, columns + tile * 128 + k * 8, low + at, kSumDesc, k > 0 || add ? 1u : 0u);
+        }
+        if (last)
+          umma_commit(&bars[kBarValueLowFree]);
+        add = true;
+      }
 #pragma unroll
       for (int k = 0; k < kTileTokens / 16; ++k) {
         const uint32_t at = (k / 4) * ((kDim * 128) >> 4) + (k % 4) * 2;
         umma_f16_ts(columns + 256 + tile * kDim, columns + tile * 128 + k * 8, b + at, kSumDesc, k > 0 || add ? 1u : 0u);
       }
       umma_commit(&bars[kBarSums + tile]);
+      if (last)
+        umma_commit(&bars[kBarValueFree + stage]);
     };
-    bool good = wait(kBarQuery, 0) && wait(kBarKeyFull, 0) && (!kExact || wait(kBarLowFull, 0));
+    bool good = wait(kBarQuery, 0) && wait(kBarKeyFull, 0) && (MODE == kRounded || wait(kBarKeyLowFull, 0));
     tcgen05_fence_after_thread_sync();
     if (good && leader) {
       for (int i = 0; i < tiles_q; ++i)
@@ -811,20 +861,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_kernel(const __gri
     }
 #pragma unroll 1
     for (int j = 0; j < tiles && good; ++j) {
-      const int stage = j & 1, next = (j + 1) & 1;
-      good = wait(kBarValueFull + stage, j >> 1);
+      const int next = (j + 1) % L::kKeyStages;
+      good = wait(kBarValueFull + (j & 1), j >> 1) && (MODE != kExactAll || wait(kBarValueLowFull, j));
       for (int i = 0; i < tiles_q && good; ++i) {
         good = wait(kBarWeights + i, j);
         tcgen05_fence_after_thread_sync();
-        if (good && leader) {
-          sum(i, stage, j > 0);
-          if (i == tiles_q - 1)
-            umma_commit(&bars[kBarValueFree + stage]);
-        }
+        if (good && leader)
+          sum(i, j & 1, j > 0, i == tiles_q - 1);
         __syncwarp();
         if (j + 1 < tiles) {
           if (i == 0 && good)
-            good = wait(kBarKeyFull + next, (j + 1) >> 1) && (!kExact || wait(kBarLowFull, j + 1));
+            good = wait(kBarKeyFull + next, (j + 1) / L::kKeyStages) && (MODE == kRounded || wait(kBarKeyLowFull, j + 1));
           tcgen05_fence_after_thread_sync();
           if (good && leader)
             score(i, next, i == tiles_q - 1);
