@@ -392,7 +392,10 @@ int tcrv_cuda_gemm_q4_0_q8_0_static_scratch(size_t n, float *s, const uint8_t *v
  * What lies between a decoder layer's projections in a serving step: which slots the step's new
  * tokens get, rotary positions, the cache's writer, and attention over it.  The reference has none
  * of these operations.  Activations are f32, fp16 or bf16; every sum, soft-max statistic and
- * rotation is f32 or wider.  No entry allocates; all may be captured into a graph. */
+ * rotation is f32 or wider.  Tensor-core operands of 16-bit attention calls are rounded to fp16, half a
+ * step of 2^-11 of each: soft-max weights (times the value's scale, or not), and for bf16 requests of more
+ * than 32 rows (new tokens * heads / kv_heads) with heads of 64 or 128 the values, and without lse the keys;
+ * operands of f32 calls are two fp16 terms, 2^-22.  No entry allocates; all may be captured into a graph. */
 #define TCRV_CUDA_TYPE_F32 0
 #define TCRV_CUDA_TYPE_F16 1
 #define TCRV_CUDA_TYPE_BF16 2

@@ -11,7 +11,11 @@ namespace {
 
 using namespace attention;
 
-// Rows of a request (new tokens * query heads of a kv head) from which its rows go to the prefill kernel, where there is one.
+// Rows of a request (new tokens * query heads of a kv head) from which its rows go to the prefill kernel, where there is one.  Contexts
+// of 4096, 32 / 8 heads of 128, cold caches, columns kernel against prefill (bf16; bf16 with lse; fp16), us: 16 requests of 20 rows 83
+// against 95 (bf16), of 32 rows 112 against 97, of 36 rows 140 against 93; 116; 126, of 64 rows 198 against the same; 64 requests of
+// 20 rows 253 against 312, of 32 rows 372 against 314, of 36 rows 474 against 302; 392; 437; one request, whose few row blocks leave
+// SMs idle, of 32 rows 26 against 41, of 64 rows 36 against 43; 45; 47, of 128 rows 46 against 45.
 constexpr size_t kPrefillRows = 33;
 
 struct Shape {
@@ -47,7 +51,10 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   s.bytes = s.columns_bytes;
   if (s.prefill) {
     const size_t items = (all + 2 * kTileRows - 1) / (2 * kTileRows) * c.requests * c.cache.kv_heads;
-    // with fewer row blocks than half the SMs, each one's tokens are shared by several CTAs
+    // With fewer row blocks than half the SMs, each one's tokens are shared by several CTAs, of at least 4 tiles each (64 tokens
+    // behind 32768, whole and shared: 689 us, 80; 512 behind 3584: 114, 81).  From half the SMs on the join costs more than idle SMs
+    // (1024 behind 3072: 116, 154 shared).  At least one tile instead of 4: 64 behind 4032 45 us instead of 54, others the same or
+    // a little more; up to 148 parts instead of 32: 131072 tokens of one kv head 116 instead of 131, 32768 74 instead of 69.
     const size_t tiles = (c.width * c.cache.groups + kTileGroups - 1) / kTileGroups;
     size_t splits = items * 2 > static_cast<size_t>(sm_count()) ? 1 : sm_count() / items;
     splits = splits > (tiles + 3) / 4 ? (tiles + 3) / 4 : splits;

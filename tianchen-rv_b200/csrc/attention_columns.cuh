@@ -13,7 +13,7 @@
 // (lifted by a power of two that brings the largest scale seen so far into [2^14, 2^15)):
 //   fp16 and bf16 calls: both to one fp16 term, half a step of 2^-11 (a 16-bit query is exact);
 //   f32 calls: both to two fp16 terms, 2^-22 relative, with a product each into the same sums, or up to 4
-//   rows with a column each (777 tokens, 4 rows: 19 us against 15).
+//   rows with a column each (4 rows, cold caches: 777 tokens 19.5 us against 15.4, 64 x 2048 tokens 87 against 65).
 // A weight times its scale leaves fp16's normal range below 2^-28 of the largest scale: what it then loses is at most 2^-39 of that
 // scale.  (Without a lift values of 1e-4 lost a percent, and those beside a token e^8 above them more.)
 // Maximum, sum and accumulators are f32.
@@ -31,8 +31,9 @@ constexpr int kUnitGroups = 2;                             // groups of 16 token
 constexpr int kUnitTokens = kUnitGroups * kGroupTokens;
 constexpr int kCombineThreads = 128;
 // What the end of a segment costs a CTA, in units: its warps wait for the last of them and join their parts.  Counted into the
-// list that is cut into ranges, or the CTAs among short contexts end last (64 requests of up to 8191 tokens: 128 us without, 118
-// with 8, 109 with 16 to 24, 113 with 40; 16 x 5 drafted tokens: 93, then 72, 76).
+// list that is cut into ranges, or the CTAs among short contexts end last.  With 8, 20 and 40, us, cold caches: 64 requests of up to
+// 8191 tokens, bf16, heads of 64: 91, 87, 91, of 128: 132, 122, 128, of 256: 247, 216, 218, f32 114, 110, 114; 16 x 5 drafted tokens,
+// f32: 87, 79, 85, bf16: 83, 75, 77.
 constexpr int kSegmentUnits = 20;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -362,11 +363,12 @@ __device__ __forceinline__ void write_row(const tcrv_cuda_attention_call &c, siz
 // segment that lies in one range is finished there; of one that does not, each CTA leaves maximum, sum and
 // accumulators in the workspace for the combine kernel.
 //
-// Bound by instructions, not by the 9/16 byte a value: a warp's unit of D = 128 and 8 rows takes about 880 (32 words unpacked
-// at 9 each, 32 products, the weights of each block, the soft-max, the copies' addresses), issued in 59 % of the cycles by 16
-// warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 87 us, 3.5 TB/s of cache; with (w & mask) | bits left to the compiler as two
-// instructions, products that add to zeroed registers, and 64-bit cursors, 1100 instructions and 112 us.  Rows of several
-// tiles share a unit's unpacking (NT); their accumulators leave room for one CTA of 8 warps on an SM from 16 rows of 128 on.
+// Bound by instructions, not by the 9/16 byte a value: a warp's unit of D = 128 and 8 rows takes about 930 (32 words unpacked
+// at 9 each, 32 products, the weights of each block, the soft-max, the scales' lift, the copies' addresses), issued in 60 % of the
+// cycles by 16 warps.  2 x 131072 tokens, 32 / 8 heads, fp16: 93 us, 3.2 TB/s of cache; with (w & mask) | bits left to the compiler
+// as two instructions, products that add to zeroed registers, and 64-bit cursors 200 instructions and a quarter more.  Rows of
+// several tiles share a unit's unpacking (NT); their accumulators leave room for one CTA of 8 warps on an SM from 16 rows of 128 on,
+// which covers no latencies: 16 x 5 drafted tokens, f32, 70 us with 30 % of the issue slots used.
 template <int NB, int NT, int MODE>
 __global__ void __launch_bounds__(kThreads, NB *NT <= 4 ? 2 : 1) columns_kernel(const __grid_constant__ ColumnParams p) {
   using L = ColumnLayout<NB, NT, MODE>;

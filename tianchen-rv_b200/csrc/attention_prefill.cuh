@@ -7,11 +7,14 @@
 // Warps 0..7 are the soft-max, of one tile after the other: two threads to a row, 64 columns each; warps 8..15 turn quants into the fp16
 // operands in shared memory, warp 16 issues the products.  While one tile's soft-max runs the other tile's products do.
 //
-// What bounds it: the soft-max warps, which never wait (a step of one tile takes them about 2100 cycles, 1024 of them the
-// exponential unit's; the tensor cores are busy 35 to 40 % of the time).  4 prompts of up to 2048 tokens behind contexts of up to
-// 2048, 32 / 8 heads of 128, bf16: 453 us, 675 TFLOP/s of the pairs that count.  Measured on the way: four warps unpacking instead
-// of eight 818 us; a thread to a row, one warpgroup to a tile, 459 (with the tiles' passes taking turns 510); half of the
-// exponentials by a polynomial 517, for the schedulers have no cycles to spare for it.
+// What bounds it: the soft-max warps (a step of one tile takes them about 2100 SM cycles, 1024 of them the exponential unit's, and
+// 2490 with keys whole, see below, for shared memory and issue slots are shared with twice the key operands); with values whole too
+// 3070, the products of one tile no longer fitting behind the other's soft-max.  Besides its steps a CTA pays for its query rows, its
+// first groups and its results, together as much as about eight pairs of steps when caches are cold.  4 prompts of up to 2048 tokens behind contexts of up
+// to 2048, 32 / 8 heads of 128: bf16 450 us, 680 TFLOP/s of the pairs that count, with lse 510, fp16 567 (428 without second operands,
+// 470 with the keys' alone).  Measured on the way, bf16 without second operands: four warps unpacking instead of eight 818 us; a thread
+// to a row, one warpgroup to a tile, 459 (with the tiles' passes taking turns 510); half of the exponentials by a polynomial 517, for
+// the schedulers have no cycles to spare for it.
 //
 // Numbers.  Key and value operands are d * (n - 8) rounded to fp16 (half a step of 2^-11), for their f32 sums could not be scaled
 // block by block without reading S and O once for every block of 32.  What the rounding leaves out is a multiple of the scale's
