@@ -495,13 +495,15 @@ int tcrv_cuda_kv_plan(const tcrv_cuda_kv_plan_call *call, tcrv_cuda_stream strea
  * first_rows[r] .. first_rows[r+1] - 1 (without first_rows: row r alone), the last tokens of the
  * kv_lens[r] that it has in the pages block_table[r * table_stride ..]; row i of n sees the tokens up to
  * its own position kv_lens[r] - n + i and, if window > 0, only the last `window` of those.  Rows from
- * max_new on and rows behind `rows` are left out; the others keep their positions.  heads is a multiple of kv_heads, query heads h * (heads / kv_heads) .. share kv head h.
+ * max_new on and rows behind `rows` are left out; the others keep their positions.  heads is a multiple
+ * of kv_heads, query heads h * (heads / kv_heads) .. share kv head h.
  * A row that sees nothing gets zeros and lse = -inf; rows outside every request are left as they were.
- * Tokens behind `width` pages and tokens in pages outside the cache count as unseen.  `lse` (may be
- * null) gets the natural logarithm of each row's soft-max sum, [row][head].  Strides count elements,
- * the elements of a head are adjacent; out == q with equal strides works in place, any other overlap of
- * the two is refused (with unequal strides all between first and last byte counts).  dim: 64, 96, 128,
- * 192 or 256.
+ * Tokens behind `width` pages and tokens in pages outside the cache count as unseen.  A scale that is an
+ * infinity or a NaN reaches only rows that see its token: a key's all of the row, a value's the 32
+ * elements of its block.  `lse` (may be null) gets the natural logarithm of each row's soft-max sum,
+ * [row][head].  Strides count elements, the elements of a head are adjacent; out == q with equal strides
+ * works in place, any other overlap of the two is refused (with unequal strides all between first and
+ * last byte counts).  dim: 64, 96, 128, 192 or 256.
  * `workspace` holds the partial results of contexts that are split: 256-byte aligned,
  * tcrv_cuda_attention_q4_0_workspace_bytes(call) bytes (which ignores the call's pointers); nothing in
  * it outlives the call, and calls that may run at the same time need one each. */
