@@ -51,10 +51,11 @@ Shape shape_of(const tcrv_cuda_attention_call &c) {
   s.bytes = s.columns_bytes;
   if (s.prefill) {
     const size_t items = (all + 2 * kTileRows - 1) / (2 * kTileRows) * c.requests * c.cache.kv_heads;
-    // With fewer row blocks than half the SMs, each one's tokens are shared by several CTAs, of at least 4 tiles each (64 tokens
-    // behind 32768, whole and shared: 689 us, 80; 512 behind 3584: 114, 81).  From half the SMs on the join costs more than idle SMs
-    // (1024 behind 3072: 116, 154 shared).  At least one tile instead of 4: 64 behind 4032 45 us instead of 54, others the same or
-    // a little more; up to 148 parts instead of 32: 131072 tokens of one kv head 116 instead of 131, 32768 74 instead of 69.
+    // With fewer row blocks than half the SMs, each one's tokens are shared by several CTAs, of at least 4 tiles each (the last 64
+    // tokens of 32768, whole and shared: 689 us, 80; the last 512 of 4096: 114, 81).  From half the SMs on the join costs more than
+    // idle SMs (the last 1024 of 4096: 116, 154 shared).  At least one tile instead of 4: the last 64 of 4096 45 us instead of 54,
+    // others the same or a little more; up to 148 parts instead of 32: 131072 tokens of one kv head 116 instead of 131, 32768 74
+    // instead of 69.
     const size_t tiles = (c.width * c.cache.groups + kTileGroups - 1) / kTileGroups;
     size_t splits = items * 2 > static_cast<size_t>(sm_count()) ? 1 : sm_count() / items;
     splits = splits > (tiles + 3) / 4 ? (tiles + 3) / 4 : splits;
